@@ -1,0 +1,772 @@
+// A paged cache of keys and values: rows appended to it, and attention of a few new tokens over it.
+//
+// Cache: keys and values [pages, page_size, kv_heads, D] each (any strides with contiguous heads' elements); a sequence's token
+// j lies in page block_table[b, j / page_size], row j % page_size.
+#include "common.cuh"
+#include "ptx.cuh"
+#include <math_constants.h>
+#include <type_traits>
+
+namespace i4tc {
+
+namespace {
+
+constexpr unsigned kStatusRange = 4u;   // status word: a block table entry, a length or an index out of range
+
+// ---- append ------------------------------------------------------------------------------------------------------------
+// Row i < counts[b] of sequence b, taken from new row select[b, i] (i without select), goes to token lengths[b] + i.  Bound: the rows
+// read and written once.  A block takes a few rows; their places are looked up once, by a thread each.
+constexpr int kAppendThreads = 256;
+
+struct AppendParams {
+  const void *k, *v;
+  void *k_cache, *v_cache;
+  long long new_batch, new_token, new_head, page_stride, slot_stride, head_stride;   // bytes
+  const int *table, *lengths, *counts, *select;
+  long long table_stride, select_stride;
+  int batch, tokens, heads, row_units;   // row_units: accesses of one head
+  int pages, page_size, table_width;
+  int rows_each;                         // of a block
+  unsigned int* status;
+};
+
+template <typename V>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendParams p) {
+  __shared__ long long from[kAppendThreads], to[kAppendThreads];
+  pdl_wait();
+  const long long row0 = (long long)blockIdx.x * p.rows_each, rows = (long long)p.batch * p.tokens;
+  const int n = (int)min((long long)p.rows_each, rows - row0);
+  if (threadIdx.x < n) {
+    const long long row = row0 + threadIdx.x;
+    const int b = (int)(row / p.tokens), i = (int)(row - (long long)b * p.tokens);
+    const int count = p.counts ? p.counts[b] : p.tokens;
+    long long src = -1, dst = -1;
+    bool bad = count < 0 || count > p.tokens;
+    if (i < count && !bad) {
+      const int pick = p.select ? p.select[b * p.select_stride + i] : i;
+      const long long at = (long long)p.lengths[b] + i;
+      bad = pick < 0 || pick >= p.tokens || at < i || at >= (long long)p.table_width * p.page_size;
+      if (!bad) {
+        const int slot = (int)(at % p.page_size), page = p.table[b * p.table_stride + at / p.page_size];
+        bad = page < 0 || page >= p.pages;
+        if (!bad) {
+          src = b * p.new_batch + pick * p.new_token;
+          dst = page * p.page_stride + slot * p.slot_stride;
+        }
+      }
+    }
+    if (bad) atomicOr(p.status, kStatusRange);
+    from[threadIdx.x] = src;
+    to[threadIdx.x] = dst;
+  }
+  __syncthreads();
+  const int per_row = 2 * p.heads * p.row_units;   // keys, then values
+  for (int i = threadIdx.x; i < n * per_row; i += kAppendThreads) {
+    const int r = i / per_row, j = i - r * per_row;
+    if (to[r] < 0) continue;
+    const bool value = j >= per_row / 2;
+    const int c = value ? j - per_row / 2 : j, head = c / p.row_units, unit = c - head * p.row_units;
+    const char* src = static_cast<const char*>(value ? p.v : p.k) + from[r] + head * p.new_head;
+    char* dst = static_cast<char*>(value ? p.v_cache : p.k_cache) + to[r] + head * p.head_stride;
+    reinterpret_cast<V*>(dst)[unit] = reinterpret_cast<const V*>(src)[unit];
+  }
+}
+
+// ---- attention ---------------------------------------------------------------------------------------------------------
+//   out[b, t, h] = sum_j w_j v_j / sum_j w_j,  w_j = exp(scale * q[b, t, h] . k_j)
+// over the lengths[b] cached tokens of the sequence and those new tokens j that mask[b, t, j] names (the first t + 1 without a mask);
+// nothing visible gives zeros.  Query heads h of one group (heads / kv_heads) read the same keys and values.
+//
+// Bound: keys and values of the cache, read once: the T new tokens of the heads of a group are the rows of one tile, so a
+// key's 2 D bytes serve T * group rows (64 at sixteen drafts of four heads: 64 operations a byte, below what mma.sync gives; a
+// tcgen05 tile of 128 rows would be padding for nearly all trees).  One pass with the running maximum and sum of the softmax.
+//
+// The work is 64-key tiles.  The tiles of all sequences, heads and row tiles stand in one line, which is cut into equal parts,
+// one a block: ragged lengths, one long sequence and many short ones all keep every block busy alike.  A part begins and
+// ends anywhere; what it holds of an item (sequence, kv head, row tile) goes out as the result where it holds all of it, else
+// as maximum, sum and weighted values (fp32) to scratch, and a second kernel adds an item's parts in ascending order.  No
+// atomics: the same bits in every run.
+//
+// A block's four warps are WR row warps (16 rows each) times 4 / WR key warps, which share out a tile's keys and are added at the
+// item's end: few rows do not leave warps idle.  Tiles arrive by cp.async, two ahead; a key's address (its page) is looked
+// up one tile before that.
+constexpr int kTile = 64, kStages = 3, kAttendThreads = 128, kPlaces = 4;
+
+struct AttendParams {
+  const void *q, *k, *v, *k_cache, *v_cache;
+  const int *table, *lengths;
+  const uint8_t* mask;
+  void* out;
+  float* scratch;
+  long long q_batch, q_token, q_head, new_batch, new_token, new_head, page_stride, slot_stride, head_stride;   // elements
+  long long table_stride, mask_batch;
+  int batch, tokens, heads, kv_heads, group, D;
+  int pages, page_size, table_width;
+  int rows, row_tiles;          // of an item: tokens * group
+  int parts;                    // blocks
+  float scale_log2;             // scale * log2(e)
+  unsigned int* status;
+};
+
+__device__ __forceinline__ int cached(const AttendParams& p, int b, bool report) {
+  const int n = p.lengths[b];
+  const long long most = min((long long)p.table_width * p.page_size, (long long)INT_MAX - 2 * kTile);
+  if (n >= 0 && n <= most) return n;
+  if (report) atomicOr(p.status, kStatusRange);
+  return n < 0 ? 0 : (int)most;
+}
+__device__ __forceinline__ int tiles_of(const AttendParams& p, int length) { return (length + p.tokens + kTile - 1) / kTile; }
+
+// Tiles of one (kv head, row tile) over sequences before `upto`, summed by a whole warp.
+__device__ __forceinline__ long long tiles_before(const AttendParams& p, int upto, bool report) {
+  long long n = 0;
+  for (int b = threadIdx.x & 31; b < upto; b += 32) n += tiles_of(p, cached(p, b, report));
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
+  return n;
+}
+// The sequence that holds tile `at` of the line (tiles of a sequence: its tiles times `items`), and the line's tiles before it.
+__device__ __forceinline__ int find_sequence(const AttendParams& p, long long at, int items, long long& before) {
+  const int lane = threadIdx.x & 31;
+  long long base = 0;
+  for (int b0 = 0; b0 < p.batch; b0 += 32) {
+    const long long mine = b0 + lane < p.batch ? (long long)tiles_of(p, cached(p, b0 + lane, false)) * items : 0;
+    long long incl = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+      if (lane >= o) incl += up;
+    }
+    const unsigned past = __ballot_sync(0xffffffffu, base + incl > at);
+    if (past) {
+      const int l = __ffs(past) - 1;
+      before = base + __shfl_sync(0xffffffffu, incl - mine, l);
+      return b0 + l;
+    }
+    base += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  before = base;
+  return p.batch;
+}
+__device__ __forceinline__ long long part_start(long long total, int parts, int part) { return total / parts * part + total % parts * part / parts; }
+// The part that holds tile `at`: the last whose start is not behind it.
+__device__ __forceinline__ int part_of(long long total, int parts, long long at) {
+  int lo = 0, hi = parts - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) / 2;
+    if (part_start(total, parts, mid) <= at) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+// Walks the line tile by tile.
+struct Cursor {
+  int b, item, tile, tiles, length;
+  __device__ __forceinline__ void open(const AttendParams& p) {
+    length = b < p.batch ? cached(p, b, false) : 0;
+    tiles = tiles_of(p, length);
+  }
+  __device__ __forceinline__ void next(const AttendParams& p) {
+    if (++tile < tiles) return;
+    tile = 0;
+    if (++item < p.kv_heads * p.row_tiles) return;
+    item = 0;
+    ++b;
+    open(p);
+  }
+};
+
+template <typename T>
+__device__ __forceinline__ void mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  } else {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  }
+}
+template <bool TRANS>
+__device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
+  if constexpr (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool valid) {   // zeros where not valid: nothing is read then
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16u : 0u) : "memory");
+}
+
+// Two weights in the type of the values, and what they stand for: the sum runs over the rounded weights, so that weights and sum agree.
+template <typename T>
+__device__ __forceinline__ uint32_t pack_weights(float a, float b, float& sum) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(&h);
+    sum += __uint_as_float(u << 16) + __uint_as_float(u & 0xFFFF0000u);
+    return u;
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 f = __half22float2(h);
+    sum += f.x + f.y;
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+__device__ __forceinline__ float exp2_fast(float x) {   // 2 ulp, far below the rounding of a weight
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <typename T>
+__device__ __forceinline__ uint32_t pack_out(float a, float b) {
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
+}
+// Whether any of the new tokens is visible to token t of sequence b.
+__device__ __forceinline__ bool sees_new(const AttendParams& p, int b, int t) {
+  if (p.mask == nullptr) return true;
+  const uint8_t* m = p.mask + b * p.mask_batch + (long long)t * p.tokens;
+  for (int j = 0; j < p.tokens; ++j)
+    if (m[j]) return true;
+  return false;
+}
+// 1 / sum of a row.  A sum of zero is a row that sees nothing (zeros) or one whose every score is -inf (not a number, as the formula gives).
+__device__ __forceinline__ float inverse_sum(const AttendParams& p, float sum, int b, int t, int length) {
+  if (sum != 0.f) return 1.0f / sum;
+  return length > 0 || sees_new(p, b, t) ? CUDART_NAN_F : 0.f;
+}
+
+// Scratch of a part: two slots (the item it begins in, the item it ends in) of maximum [rows], sum [rows], values [rows][DP].
+__host__ __device__ constexpr size_t slot_floats(int rows, int dp) { return (size_t)rows * (dp + 2); }
+
+template <int DP, int WR>
+struct AttendShape {
+  static constexpr int ROWS = 16 * WR, WK = 4 / WR, KEYS = kTile / WK;   // KEYS: of a tile, a warp's share
+  static constexpr int kStage = kTile * DP * 2;                          // bytes of a tile's keys, and of its values
+  static constexpr int kMerge = WK > 1 ? ROWS * (DP / 2 + 2) * 4 : 0;   // half of the elements of one key warp's rows
+  static constexpr int kSmem = kStages * 2 * kStage + kPlaces * kTile * 16 + kMerge;
+};
+
+// DP: D rounded up to 64 or 128 (the elements behind D are zeros in shared memory).
+template <typename T, int DP, int WR>
+__global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendParams p) {
+  using S = AttendShape<DP, WR>;
+  constexpr int CH = DP / 8;                        // 16-byte chunks of a row
+  constexpr int KS = DP / 16, NT = S::KEYS / 8, DT = DP / 8;
+  // weights are 2^kLift times exp(score - maximum): a fp16 weight keeps 24 + 12 bits below the largest instead of 24
+  constexpr float kLift = std::is_same_v<T, __half> ? 12.f : 0.f;
+  extern __shared__ __align__(128) uint8_t smem[];
+  const uint32_t stage0 = ptx::smem_u32(smem);
+  const char** places = reinterpret_cast<const char**>(smem + kStages * 2 * S::kStage);   // [kPlaces][kTile] keys, values
+  float* merge = reinterpret_cast<float*>(smem + kStages * 2 * S::kStage + kPlaces * kTile * 16);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int wr = warp % WR, wk = warp / WR;
+  const int g = lane >> 2, t4 = lane & 3;
+  pdl_wait();
+  pdl_trigger();
+
+  const int items = p.kv_heads * p.row_tiles;
+  const long long total = tiles_before(p, p.batch, blockIdx.x == 0) * items;
+  const int parts = (int)min((long long)p.parts, total), part = blockIdx.x;   // no part is empty
+  if (part >= parts) return;
+  const long long first = part_start(total, parts, part);
+  const int count = (int)(part_start(total, parts, part + 1) - first);
+  Cursor cur;
+  long long before;
+  cur.b = find_sequence(p, first, items, before);
+  cur.open(p);
+  cur.item = (int)((first - before) / cur.tiles);
+  cur.tile = (int)((first - before) % cur.tiles);
+  Cursor ahead = cur;                               // whose places are looked up next
+
+  // places of the tile at `ahead`: key tid of it
+  auto look_up = [&](const char*& pk, const char*& pv) {
+    pk = pv = nullptr;
+    const int j = ahead.tile * kTile + tid, head = ahead.item / p.row_tiles;
+    if (j < ahead.length) {
+      const int page = p.table[ahead.b * p.table_stride + j / p.page_size];
+      if (page >= 0 && page < p.pages) {
+        const long long at = page * p.page_stride + (j % p.page_size) * p.slot_stride + head * p.head_stride;
+        pk = static_cast<const char*>(p.k_cache) + at * 2;
+        pv = static_cast<const char*>(p.v_cache) + at * 2;
+      } else {
+        atomicOr(p.status, kStatusRange);
+      }
+    } else if (j - ahead.length < p.tokens) {
+      const long long at = ahead.b * p.new_batch + (j - ahead.length) * p.new_token + head * p.new_head;
+      pk = static_cast<const char*>(p.k) + at * 2;
+      pv = static_cast<const char*>(p.v) + at * 2;
+    }
+  };
+  auto issue = [&](int i) {                         // tile i of the part into its stage
+    const char** place = places + (i % kPlaces) * kTile * 2;
+    const uint32_t dk = stage0 + (i % kStages) * 2 * S::kStage, dv = dk + S::kStage;
+    const int c = tid % CH;
+#pragma unroll
+    for (int r = tid / CH; r < kTile; r += kAttendThreads / CH) {
+      const char *pk = place[2 * r], *pv = place[2 * r + 1];
+      const bool valid = pk != nullptr && c * 8 < p.D;
+      const uint32_t at = r * (DP * 2) + ((c ^ (r & 7)) * 16);
+      cp_async_16(dk + at, valid ? pk + c * 16 : p.k, valid);
+      cp_async_16(dv + at, valid ? pv + c * 16 : p.v, valid);
+    }
+  };
+  for (int i = 0; i < kStages && i < count; ++i) {
+    if (tid < kTile) {
+      const char *pk, *pv;
+      look_up(pk, pv);
+      places[(i * kTile + tid) * 2] = pk;
+      places[(i * kTile + tid) * 2 + 1] = pv;
+    }
+    ahead.next(p);
+  }
+  __syncthreads();
+  for (int i = 0; i < kStages - 1; ++i) {
+    if (i < count) issue(i);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+
+  uint32_t q[KS][4];
+  float o[DT][4], m[2], l[2];
+  int tok[2];                                       // of this lane's two rows; -1 behind the last
+  bool begun = true, whole = cur.tile == 0;         // begun: the item's rows have to be set up; whole: this part has it from its start
+
+  for (int i = 0; i < count; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    __syncthreads();
+    if (i + kStages - 1 < count) issue(i + kStages - 1);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    const char *pk = nullptr, *pv = nullptr;
+    const bool more = i + kStages < count;
+    if (more && tid < kTile) look_up(pk, pv);
+
+    if (begun) {
+      const int row0 = (cur.item % p.row_tiles) * S::ROWS + wr * 16 + g, kvh = cur.item / p.row_tiles;
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = row0 + 8 * h;
+        tok[h] = row < p.rows ? row / p.group : -1;
+        const T* src = static_cast<const T*>(p.q) + cur.b * p.q_batch + (long long)(row / p.group) * p.q_token +
+                       (long long)(kvh * p.group + row % p.group) * p.q_head;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int d = ks * 16 + e * 8 + 2 * t4;
+            q[ks][2 * e + h] = tok[h] >= 0 && d < p.D ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
+          }
+        m[h] = -CUDART_INF_F;
+        l[h] = 0.f;
+      }
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) o[dt][k] = 0.f;
+      begun = false;
+    }
+
+    const uint32_t sk = stage0 + (i % kStages) * 2 * S::kStage, sv = sk + S::kStage;
+    const int key0 = wk * S::KEYS;                  // of this warp, in the tile
+    float s[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[nt][k] = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+      for (int np = 0; np < NT / 2; ++np) {
+        uint32_t b[4];
+        const int row = key0 + np * 16 + (lane & 7) + ((lane >> 4) & 1) * 8, c = ks * 2 + ((lane >> 3) & 1);
+        ldmatrix4<false>(b, sk + row * (DP * 2) + ((c ^ (row & 7)) * 16));
+        mma<T>(s[2 * np], q[ks], b[0], b[1]);
+        mma<T>(s[2 * np + 1], q[ks], b[2], b[3]);
+      }
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) s[nt][k] *= p.scale_log2;
+    const int j0 = cur.tile * kTile;
+    const bool edge = j0 + kTile > cur.length;      // the tile holds new tokens, or what is behind them
+    bool odd = false;
+    if (edge) {
+      // not only the scores of what a row does not see: its values may be infinite or no numbers, which a weight of zero does not undo
+      for (int r = tid; r < kTile * CH; r += kAttendThreads) {
+        const int key = r / CH, c = r % CH;
+        if (j0 + key < cur.length) continue;
+        const uint32_t at = sv + key * (DP * 2) + ((c ^ (key & 7)) * 16);
+        uint4 v = ptx::lds128(at);
+        uint32_t* u = &v.x;
+        bool hit = false;
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            constexpr uint32_t kExp = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
+            if (((u[k] >> (16 * half)) & kExp) == kExp) {
+              u[k] &= half ? 0x0000FFFFu : 0xFFFF0000u;
+              hit = true;
+            }
+          }
+        if (hit) {
+          ptx::sts128(at, v);
+          odd = true;
+        }
+      }
+      odd = __syncthreads_or(odd);
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const int j = j0 + key0 + nt * 8 + 2 * t4 + (k & 1) - cur.length, t = tok[k >> 1];
+          bool seen = j < 0;
+          if (j >= 0 && j < p.tokens && t >= 0)
+            seen = p.mask ? p.mask[cur.b * p.mask_batch + (long long)t * p.tokens + j] != 0 : j <= t;
+          if (!seen) s[nt][k] = -CUDART_INF_F;
+        }
+    }
+
+    float top[2] = {m[0], m[1]};
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) top[k >> 1] = fmaxf(top[k >> 1], s[nt][k]);
+    float base[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
+      top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
+      base[h] = top[h] == -CUDART_INF_F ? 0.f : top[h] - kLift;
+      const float fade = exp2_fast(m[h] - (base[h] + kLift));
+      m[h] = top[h];
+      l[h] *= fade;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        o[dt][2 * h] *= fade;
+        o[dt][2 * h + 1] *= fade;
+      }
+    }
+    if (odd) {                                      // what was taken out of the values goes to the rows that see it
+      for (int key = key0; key < key0 + S::KEYS; ++key) {
+        const int j = j0 + key - cur.length;
+        if (j < 0 || j >= p.tokens) continue;
+        const T* src = static_cast<const T*>(p.v) + cur.b * p.new_batch + j * p.new_token + (long long)(cur.item / p.row_tiles) * p.new_head;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int t = tok[h];
+          if (t < 0 || !(p.mask ? p.mask[cur.b * p.mask_batch + (long long)t * p.tokens + j] != 0 : j <= t)) continue;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int d = dt * 8 + 2 * t4 + e;
+              if (d < p.D) {
+                const float x = to_f32(src[d]);
+                if (!isfinite(x)) o[dt][2 * h + e] += x;
+              }
+            }
+        }
+      }
+    }
+    uint32_t w[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        w[nt][h] = pack_weights<T>(exp2_fast(s[nt][2 * h] - base[h]), exp2_fast(s[nt][2 * h + 1] - base[h]), l[h]);
+#pragma unroll
+    for (int kk = 0; kk < NT / 2; ++kk) {
+      const uint32_t a[4] = {w[2 * kk][0], w[2 * kk][1], w[2 * kk + 1][0], w[2 * kk + 1][1]};
+#pragma unroll
+      for (int dp = 0; dp < DT / 2; ++dp) {
+        uint32_t b[4];
+        const int row = key0 + kk * 16 + (lane & 15), c = dp * 2 + (lane >> 4);
+        ldmatrix4<true>(b, sv + row * (DP * 2) + ((c ^ (row & 7)) * 16));
+        mma<T>(o[2 * dp], a, b[0], b[1]);
+        mma<T>(o[2 * dp + 1], a, b[2], b[3]);
+      }
+    }
+
+    const bool ends = cur.tile + 1 == cur.tiles;
+    if (ends || i + 1 == count) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+      }
+      if constexpr (S::WK > 1) {
+        // the key warps, one after the other and half of the elements at a time, into the first
+        float* mo = merge + (wr * 16 + g) * (DP / 2) + 2 * t4;
+        float* ml = merge + S::ROWS * (DP / 2) + (wr * 16 + g) * 2;
+        for (int from = 1; from < S::WK; ++from) {
+          float fa[2], fb[2];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            __syncthreads();
+            if (wk == from) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+#pragma unroll
+                for (int dt = 0; dt < DT / 2; ++dt)
+                  *reinterpret_cast<float2*>(mo + 8 * h * (DP / 2) + dt * 8) =
+                      make_float2(o[half * (DT / 2) + dt][2 * h], o[half * (DT / 2) + dt][2 * h + 1]);
+                if (half == 0 && t4 == 0) *reinterpret_cast<float2*>(ml + 16 * h) = make_float2(m[h], l[h]);
+              }
+            }
+            __syncthreads();
+            if (wk == 0) {
+#pragma unroll
+              for (int h = 0; h < 2; ++h) {
+                if (half == 0) {
+                  const float2 his = *reinterpret_cast<const float2*>(ml + 16 * h);
+                  const float both = fmaxf(m[h], his.x), zero = both == -CUDART_INF_F ? 0.f : both;
+                  fa[h] = exp2_fast(m[h] - zero);
+                  fb[h] = exp2_fast(his.x - zero);
+                  m[h] = both;
+                  l[h] = l[h] * fa[h] + his.y * fb[h];
+                }
+#pragma unroll
+                for (int dt = 0; dt < DT / 2; ++dt) {
+                  const float2 v = *reinterpret_cast<const float2*>(mo + 8 * h * (DP / 2) + dt * 8);
+                  float* mine = o[half * (DT / 2) + dt] + 2 * h;
+                  mine[0] = mine[0] * fa[h] + v.x * fb[h];
+                  mine[1] = mine[1] * fa[h] + v.y * fb[h];
+                }
+              }
+            }
+          }
+        }
+      }
+      if (wk == 0) {
+        const int row0 = (cur.item % p.row_tiles) * S::ROWS + wr * 16 + g, kvh = cur.item / p.row_tiles;
+        if (whole && ends) {
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int row = row0 + 8 * h;
+            if (tok[h] < 0) continue;
+            const float inv = inverse_sum(p, l[h], cur.b, tok[h], cur.length);
+            T* dst = static_cast<T*>(p.out) + (((long long)cur.b * p.tokens + tok[h]) * p.heads + kvh * p.group + row % p.group) * p.D;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) {
+              const int d = dt * 8 + 2 * t4;
+              if (d < p.D) *reinterpret_cast<uint32_t*>(dst + d) = pack_out<T>(o[dt][2 * h] * inv, o[dt][2 * h + 1] * inv);
+            }
+          }
+        } else {
+          // the item the part began in, or (where that is another) the one it ends in
+          const bool opening = !whole || i == cur.tile;
+          float* slot = p.scratch + ((size_t)part * 2 + (opening ? 0 : 1)) * slot_floats(S::ROWS, DP);
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const int row = wr * 16 + g + 8 * h;
+            if (t4 == 0) {
+              slot[row] = m[h];
+              slot[S::ROWS + row] = l[h];
+            }
+            float* dst = slot + 2 * S::ROWS + row * DP + 2 * t4;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float2*>(dst + dt * 8) = make_float2(o[dt][2 * h], o[dt][2 * h + 1]);
+          }
+        }
+      }
+      begun = whole = true;
+    }
+    cur.next(p);
+    if (more) {
+      if (tid < kTile) {
+        const int at = ((i + kStages) % kPlaces) * kTile + tid;
+        places[2 * at] = pk;
+        places[2 * at + 1] = pv;
+      }
+      ahead.next(p);
+    }
+  }
+}
+
+// Items that no part held whole: their parts in ascending order.  A warp takes a row, a lane DP / 32 consecutive elements.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kAttendThreads) attend_join_kernel(const AttendParams p, int tile_rows) {
+  constexpr int E = DP / 32;
+  pdl_wait();
+  const int lane = threadIdx.x & 31;
+  const int items = p.kv_heads * p.row_tiles;
+  const int b = blockIdx.x / items, item = blockIdx.x % items;
+  const int row = blockIdx.y * (kAttendThreads / 32) + (threadIdx.x >> 5);
+  const int at_row = (item % p.row_tiles) * tile_rows + row;
+  const int length = cached(p, b, false), tiles = tiles_of(p, length);
+  const long long total = tiles_before(p, p.batch, false) * items, start = tiles_before(p, b, false) * items + (long long)item * tiles;
+  const int parts = (int)min((long long)p.parts, total);
+  const int first = part_of(total, parts, start), last = part_of(total, parts, start + tiles - 1);
+  if (first == last || row >= tile_rows || at_row >= p.rows) return;
+  const size_t step = 2 * slot_floats(tile_rows, DP);
+  const float* opening = p.scratch + first * step + (part_start(total, parts, first) == start ? 0 : step / 2);
+  auto slot = [&](int part) { return part == first ? opening : p.scratch + part * step; };
+  float top = -CUDART_INF_F;
+  for (int part = first + lane; part <= last; part += 32) top = fmaxf(top, slot(part)[row]);
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+  const float zero = top == -CUDART_INF_F ? 0.f : top;
+  float sum = 0.f, v[E];
+#pragma unroll
+  for (int e = 0; e < E; ++e) v[e] = 0.f;
+#pragma unroll 4
+  for (int part = first; part <= last; ++part) {
+    const float* s = slot(part);
+    const float f = exp2_fast(s[row] - zero);
+    sum += s[tile_rows + row] * f;
+    const float* o = s + 2 * tile_rows + row * DP + lane * E;
+    if constexpr (E == 4) {
+      const float4 x = *reinterpret_cast<const float4*>(o);
+      v[0] += x.x * f; v[1] += x.y * f; v[2] += x.z * f; v[3] += x.w * f;
+    } else {
+      const float2 x = *reinterpret_cast<const float2*>(o);
+      v[0] += x.x * f; v[1] += x.y * f;
+    }
+  }
+  const int t = at_row / p.group, head = (item / p.row_tiles) * p.group + at_row % p.group;
+  const float inv = inverse_sum(p, sum, b, t, length);
+  T* dst = static_cast<T*>(p.out) + (((long long)b * p.tokens + t) * p.heads + head) * p.D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; e += 2)
+    if (lane * E + e < p.D) *reinterpret_cast<uint32_t*>(dst + e) = pack_out<T>(v[e] * inv, v[e + 1] * inv);
+}
+
+int row_warps(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
+int padded_dim(int64_t D) { return D <= 64 ? 64 : 128; }
+int attend_parts(int sm_count, int64_t batch, int64_t items, int64_t most_length, int64_t tokens) {
+  const int64_t tiles = batch * items * ((most_length + tokens + kTile - 1) / kTile), most = (int64_t)sm_count * 2;
+  return (int)(tiles < most ? tiles : most);
+}
+
+template <typename T, int DP, int WR>
+int launch_attend(const AttendParams& p, cudaStream_t st) {
+  using S = AttendShape<DP, WR>;
+  auto kernel = attend_kernel<T, DP, WR>;
+  static bool configured[64] = {false};
+  int dev = 0;
+  I4TC_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !configured[dev]) {
+    I4TC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+    if (dev < 64) configured[dev] = true;
+  }
+  I4TC_CUDA(launch_kernel(true, kernel, dim3((unsigned)p.parts), kAttendThreads, S::kSmem, st, p));
+  const dim3 grid((unsigned)(p.batch * p.kv_heads * p.row_tiles), (unsigned)((S::ROWS < p.rows ? S::ROWS : p.rows) + 3) / 4);
+  I4TC_CUDA(launch_kernel(true, attend_join_kernel<T, DP>, grid, kAttendThreads, 0, st, p, S::ROWS));
+  return I4TC_OK;
+}
+template <typename T, int DP>
+int launch_rows(const AttendParams& p, int warps, cudaStream_t st) {
+  return warps == 1 ? launch_attend<T, DP, 1>(p, st) : warps == 2 ? launch_attend<T, DP, 2>(p, st) : launch_attend<T, DP, 4>(p, st);
+}
+
+}  // namespace
+
+}  // namespace i4tc
+
+using namespace i4tc;
+
+extern "C" int64_t i4tc_tree_attention_scratch_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t D,
+                                                     int64_t most_length, int device) {
+  const DeviceInfo* info;
+  if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || D <= 0 || most_length < 0 || device_info(device, &info) != I4TC_OK) return 0;
+  const int64_t rows = tokens * (heads / kv_heads);
+  const int tile_rows = 16 * row_warps(rows);
+  const int64_t items = kv_heads * ((rows + tile_rows - 1) / tile_rows);
+  return (int64_t)attend_parts(info->sm_count, batch, items, most_length, tokens) * 2 * (int64_t)slot_floats(tile_rows, padded_dim(D)) * 4;
+}
+
+extern "C" int i4tc_tree_attention(const i4tc_tree_attention_args* a, int device, void* stream) {
+  I4TC_REQUIRE(a != nullptr, I4TC_EINVAL, "null pointer");
+  I4TC_REQUIRE(a->dtype == I4TC_BF16 || a->dtype == I4TC_FP16, I4TC_EUNSUPPORTED, "queries must be bfloat16 or float16");
+  I4TC_REQUIRE(a->batch >= 0 && a->tokens >= 0 && a->heads >= 0, I4TC_EINVAL, "bad size");
+  if (a->batch == 0 || a->tokens == 0 || a->heads == 0) return I4TC_OK;
+  I4TC_REQUIRE(a->tokens <= 64, I4TC_EUNSUPPORTED, "at most 64 new tokens a sequence");
+  I4TC_REQUIRE(a->head_dim > 0 && a->head_dim <= 128 && a->head_dim % 8 == 0, I4TC_EUNSUPPORTED,
+               "heads must have a multiple of 8 and at most 128 elements");
+  I4TC_REQUIRE(a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->heads <= 65536, I4TC_EINVAL, "heads must be a multiple of kv_heads");
+  I4TC_REQUIRE(a->batch <= 65536 && a->pages >= 0 && a->pages < (1ll << 31) && a->page_size > 0 && a->page_size < (1ll << 31) &&
+                   a->table_width >= 0 && a->table_width < (1ll << 31), I4TC_EINVAL, "bad size");
+  I4TC_REQUIRE(a->q && a->k && a->v && a->lengths && a->out && a->scratch, I4TC_EINVAL, "null pointer");
+  I4TC_REQUIRE(a->table_width == 0 || a->pages == 0 || (a->k_cache && a->v_cache && a->block_table), I4TC_EINVAL, "null pointer");
+  I4TC_REQUIRE(aligned_to(a->k, 16) && aligned_to(a->v, 16) && aligned_to(a->k_cache, 16) && aligned_to(a->v_cache, 16) &&
+                   aligned_to(a->q, 4) && aligned_to(a->out, 16) && aligned_to(a->scratch, 16) && a->q_batch % 2 == 0 && a->q_token % 2 == 0 &&
+                   a->q_head % 2 == 0 && (a->new_batch | a->new_token | a->new_head | a->page_stride | a->slot_stride | a->head_stride) % 8 == 0,
+               I4TC_EALIGN, "keys and values must be 16-byte aligned, and queries 4-byte");
+  const DeviceInfo* info;
+  if (int rc = device_info(device, &info)) return rc;
+  I4TC_REQUIRE(info->cc_major == 10, I4TC_EDEVICE, "device %d is sm_%d%d; this library needs sm_100", device, info->cc_major, info->cc_minor);
+  AttendParams p = {};
+  p.q = a->q; p.k = a->k; p.v = a->v; p.k_cache = a->k_cache; p.v_cache = a->v_cache;
+  p.table = a->block_table; p.lengths = a->lengths; p.mask = a->mask; p.out = a->out; p.scratch = static_cast<float*>(a->scratch);
+  p.q_batch = a->q_batch; p.q_token = a->q_token; p.q_head = a->q_head;
+  p.new_batch = a->new_batch; p.new_token = a->new_token; p.new_head = a->new_head;
+  p.page_stride = a->page_stride; p.slot_stride = a->slot_stride; p.head_stride = a->head_stride;
+  p.table_stride = a->table_stride; p.mask_batch = a->mask_batch;
+  p.batch = (int)a->batch; p.tokens = (int)a->tokens; p.heads = (int)a->heads; p.kv_heads = (int)a->kv_heads;
+  p.group = p.heads / p.kv_heads; p.D = (int)a->head_dim;
+  p.pages = (int)a->pages; p.page_size = (int)a->page_size; p.table_width = (int)a->table_width;
+  const int64_t rows = (int64_t)p.tokens * p.group;
+  const int warps = row_warps(rows);
+  p.rows = (int)rows; p.row_tiles = (int)((rows + 16 * warps - 1) / (16 * warps));
+  const int64_t items = (int64_t)p.kv_heads * p.row_tiles;
+  I4TC_REQUIRE(a->batch * items < (1ll << 31), I4TC_EINVAL, "too many heads");
+  const int64_t most_length = a->table_width * a->page_size;
+  p.parts = attend_parts(info->sm_count, a->batch, items, most_length, a->tokens);
+  I4TC_REQUIRE(a->scratch_bytes >= (int64_t)p.parts * 2 * (int64_t)slot_floats(16 * warps, padded_dim(p.D)) * 4, I4TC_EWORKSPACE, "the scratch is too small");
+  p.scale_log2 = (float)(a->scale * 1.4426950408889634);
+  p.status = info->status;
+  DeviceGuard guard(device);
+  I4TC_CUDA(guard.err);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto pick = [&](auto type) {
+    using T = decltype(type);
+    return padded_dim(p.D) == 64 ? launch_rows<T, 64>(p, warps, st) : launch_rows<T, 128>(p, warps, st);
+  };
+  return a->dtype == I4TC_BF16 ? pick(__nv_bfloat16{}) : pick(__half{});
+}
+
+extern "C" int i4tc_kv_append(const i4tc_kv_append_args* a, int device, void* stream) {
+  I4TC_REQUIRE(a != nullptr, I4TC_EINVAL, "null pointer");
+  I4TC_REQUIRE(a->element_bytes == 2, I4TC_EUNSUPPORTED, "keys and values must be bfloat16 or float16");
+  I4TC_REQUIRE(a->batch >= 0 && a->tokens >= 0 && a->kv_heads >= 0 && a->head_dim >= 0, I4TC_EINVAL, "bad size");
+  if (a->batch == 0 || a->tokens == 0 || a->kv_heads == 0 || a->head_dim == 0) return I4TC_OK;
+  I4TC_REQUIRE(a->batch < (1ll << 31) && a->tokens < (1ll << 31) && a->kv_heads <= 65536 && a->head_dim <= 2048 && a->pages >= 0 &&
+                   a->pages < (1ll << 31) && a->page_size > 0 && a->page_size < (1ll << 31) && a->table_width >= 0 && a->table_width < (1ll << 31),
+               I4TC_EINVAL, "bad size");
+  I4TC_REQUIRE(a->k && a->v && a->lengths, I4TC_EINVAL, "null pointer");
+  I4TC_REQUIRE(a->table_width == 0 || a->pages == 0 || (a->k_cache && a->v_cache && a->block_table), I4TC_EINVAL, "null pointer");
+  const DeviceInfo* info;
+  if (int rc = device_info(device, &info)) return rc;
+  AppendParams p = {};
+  p.k = a->k; p.v = a->v; p.k_cache = a->k_cache; p.v_cache = a->v_cache;
+  p.new_batch = a->new_batch * 2; p.new_token = a->new_token * 2; p.new_head = a->new_head * 2;
+  p.page_stride = a->page_stride * 2; p.slot_stride = a->slot_stride * 2; p.head_stride = a->head_stride * 2;
+  p.table = a->block_table; p.lengths = a->lengths; p.counts = a->counts; p.select = a->select;
+  p.table_stride = a->table_stride; p.select_stride = a->select_stride;
+  p.batch = (int)a->batch; p.tokens = (int)a->tokens; p.heads = (int)a->kv_heads;
+  p.pages = (int)a->pages; p.page_size = (int)a->page_size; p.table_width = (int)a->table_width;
+  p.status = info->status;
+  int bytes = 16;   // the widest access that strides, rows and addresses are multiples of
+  const long long all = p.new_batch | p.new_token | p.new_head | p.page_stride | p.slot_stride | p.head_stride | a->head_dim * 2;
+  while (bytes > 2 && (all % bytes != 0 || !aligned_to(p.k, bytes) || !aligned_to(p.v, bytes) || !aligned_to(p.k_cache, bytes) || !aligned_to(p.v_cache, bytes)))
+    bytes /= 2;
+  I4TC_REQUIRE(aligned_to(p.k, bytes) && aligned_to(p.v, bytes) && aligned_to(p.k_cache, bytes) && aligned_to(p.v_cache, bytes), I4TC_EALIGN,
+               "operands must be aligned to their element size");
+  p.row_units = (int)(a->head_dim * 2 / bytes);
+  const long long rows = (long long)p.batch * p.tokens, per_row = 2ll * p.heads * p.row_units;
+  p.rows_each = (int)(4 * kAppendThreads / per_row);
+  p.rows_each = p.rows_each < 1 || rows <= 2 * info->sm_count ? 1 : p.rows_each > kAppendThreads ? kAppendThreads : p.rows_each;
+  const long long blocks = (rows + p.rows_each - 1) / p.rows_each;
+  I4TC_REQUIRE(blocks < (1ll << 31) && per_row * p.rows_each < (1ll << 31), I4TC_EINVAL, "bad size");
+  DeviceGuard guard(device);
+  I4TC_CUDA(guard.err);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  auto kernel = bytes == 16 ? append_kernel<uint4> : bytes == 8 ? append_kernel<uint2> : bytes == 4 ? append_kernel<uint32_t> : append_kernel<uint16_t>;
+  I4TC_CUDA(launch_kernel(true, kernel, dim3((unsigned)blocks), kAppendThreads, 0, st, p));
+  return I4TC_OK;
+}

@@ -250,7 +250,8 @@ extern "C" int i4tc_check_status(int device, void* stream) {
   if (h != 0) {
     I4TC_CUDA(cudaMemsetAsync(info->status, 0, sizeof(unsigned int), st));
     I4TC_CUDA(cudaStreamSynchronize(st));
-    return fail(I4TC_EKERNEL, "a kernel gave up on a bounded wait (status word 0x%x)", h);
+    if (h & ~4u) return fail(I4TC_EKERNEL, "a kernel gave up on a bounded wait (status word 0x%x)", h);
+    return fail(I4TC_EKERNEL, "a length, a page of a block table or an index is out of range (status word 0x%x)", h);
   }
   return I4TC_OK;
 }

@@ -8,6 +8,9 @@ into the caller's ``out`` and return ``None`` -- the reference's ownership rules
 """
 from __future__ import annotations
 
+import math
+import struct
+
 import torch
 
 from . import _cabi
@@ -516,6 +519,231 @@ def int4_grouped_partials(a_packed, b_packed, M: int, N: int, num_groups: int) -
     return out
 
 
+# --------------------------------------------------------------------------- #
+# decoding: a few tokens over 4-bit weights and a paged cache (no reference ops)
+# --------------------------------------------------------------------------- #
+def _half_input(t: torch.Tensor, name: str, dim: int) -> None:
+    _require(isinstance(t, torch.Tensor) and t.is_cuda, f"{name} must be CUDA tensor")
+    _require(t.dim() == dim, f"{name} must be {dim}D")
+    _require(t.dtype == torch.bfloat16 or t.dtype == torch.float16, f"{name} must be bfloat16 or float16")
+    _require(not (t.requires_grad and torch.is_grad_enabled()), f"{name} requires grad: the op has no backward pass, call it under torch.no_grad()")
+
+
+def _w4a16(x: torch.Tensor, w_packed: torch.Tensor, w_scale: torch.Tensor, N: int, per_channel: bool, gated: bool, who: str) -> torch.Tensor:
+    _half_input(x, "input", 2)
+    M, K = x.shape
+    if per_channel:
+        _require(K > 0 and K % 64 == 0, "K must be a multiple of 64")
+    else:
+        _require(K > 0 and K % 128 == 0, "K must be divisible by group_size")
+    rows = 2 * N if gated else N
+    _require(w_packed.device == x.device and w_scale.device == x.device, "all tensors must be on the same device")
+    _require(w_packed.dtype == torch.uint8 and w_packed.is_contiguous(), "b_packed must be contiguous uint8")
+    _require(w_packed.numel() == rows * (K // 2), "b_packed does not have rows*K/2 bytes")
+    _require(w_scale.dtype == torch.float32 and w_scale.is_contiguous(), "scale_b must be contiguous float32")
+    _require(w_scale.numel() == (rows if per_channel else K // 128 * rows), "scale_b does not have a scale for every row (and group)")
+    ldx = x.stride(0) if M > 1 else K
+    if x.stride(1) != 1 or ldx % 8 or x.data_ptr() % 16:
+        x, ldx = x.clone(memory_format=torch.contiguous_format), K
+    out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    check(lib.i4tc_w4a16_linear(x.data_ptr(), _DTYPES[x.dtype], M, K, ldx, w_packed.data_ptr(), w_scale.data_ptr(), per_channel, gated,
+                                out.data_ptr(), N, _dev(x), _stream(x)), who)
+    return out
+
+
+def w4a16_linear(x: torch.Tensor, w_packed: torch.Tensor, w_scale: torch.Tensor, N: int, per_channel: bool = False) -> torch.Tensor:
+    """``x`` [M,K] (bf16 / fp16) times the transposed int4 weights of ``linear`` (codes [G,N,64] with scales [G,N], or [N,K/2] with [N]),
+    without quantising the activations: exact products, fp32 sums, one rounding to ``x``'s type.  [M,N].  Made for the tokens of
+    decoding: the weights are read once for every 32 of them."""
+    return _w4a16(x, w_packed, w_scale, N, per_channel, False, "w4a16_linear")
+
+
+def w4a16_gated_linear(x: torch.Tensor, w_packed: torch.Tensor, w_scale: torch.Tensor, inter: int, per_channel: bool = False) -> torch.Tensor:
+    """``silu(x Wg^T) * (x Wu^T)`` [M,inter] in one kernel: ``w4a16_linear`` over fused gate and up weights (2 * inter rows, gate
+    rows first, as ``moe_silu_mul_quant`` takes their product), with neither projection rounded before SwiGLU."""
+    return _w4a16(x, w_packed, w_scale, inter, per_channel, True, "w4a16_gated_linear")
+
+
+def rope_frequencies(rotary_dim: int, theta: float, device="cuda", scaling: str | None = None, factor: float = 1.0,
+                     trained_length: int | None = None):
+    """(frequencies float64 [rotary_dim / 2] in radians a position, scale of the rotated values) for ``rope``.
+
+    ``scaling`` stretches a context ``factor`` times: ``"linear"`` divides all positions; ``"base"`` raises ``theta`` so that the slowest
+    pair is stretched and the fastest stays; ``"by_parts"`` stretches the pairs that turn less than once within
+    ``trained_length``, keeps those that turn more than 32 times, blends in between, and scales values by ``1 + ln(factor) / 10``."""
+    _require(rotary_dim > 0 and rotary_dim % 2 == 0, "rotary_dim must be a positive even number")
+    _require(scaling in (None, "linear", "base", "by_parts"), "scaling must be None, 'linear', 'base' or 'by_parts'")
+    _require(theta > 0 and factor > 0, "theta and factor must be positive")
+    if scaling == "base":
+        _require(rotary_dim > 2, "scaling by the base needs more than one pair")
+        theta = theta * factor ** (rotary_dim / (rotary_dim - 2))
+    freqs = [theta ** (-i / rotary_dim) for i in range(0, rotary_dim, 2)]
+    scale = 1.0
+    if scaling == "linear":
+        freqs = [f / factor for f in freqs]
+    elif scaling == "by_parts":
+        _require(trained_length is not None and trained_length > 0, "scaling by parts needs trained_length")
+        keep = [min(1.0, max(0.0, (trained_length * f / (2 * math.pi) - 1) / 31)) for f in freqs]
+        freqs = [f * k + f / factor * (1 - k) for f, k in zip(freqs, keep)]
+        scale = 1.0 + 0.1 * math.log(factor) if factor > 1 else 1.0
+    return torch.tensor(freqs, dtype=torch.float64, device=device), scale
+
+
+def _rope(x, positions, freqs, interleaved, scale, inverse, in_place, who):
+    _half_input(x, "x", 3)
+    tokens, heads, D = x.shape
+    _require(positions.dim() == 1 and positions.numel() == tokens, "positions must be [tokens]")
+    _require(positions.dtype == torch.int64 or positions.dtype == torch.int32, "positions must be int32 or int64")
+    _require(freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.is_contiguous(), "freqs must be a contiguous 1D float64 tensor")
+    R = 2 * freqs.numel()
+    _require(R <= D, "a head has fewer elements than the frequencies rotate")
+    _require(positions.device == x.device and freqs.device == x.device, "all tensors must be on the same device")
+    if not positions.is_contiguous():
+        positions = positions.contiguous()
+    st, sh, sd = x.stride()
+    if in_place:
+        _require(sd == 1 or D <= 1, "elements of a head must be contiguous")
+        (near, n), (far, m) = sorted(((sh, heads), (st, tokens)), key=lambda a: (a[1] > 1, a[0]))
+        ok = (n <= 1 or near >= D) and (m <= 1 or far >= (near * (n - 1) if n > 1 else 0) + D)
+        _require(ok or x.numel() == 0, "x overlaps itself")
+        out, ot, oh = x, st, sh
+    else:
+        if sd != 1 and D > 1:
+            x = x.contiguous()
+            st, sh, sd = x.stride()
+        out = torch.empty((tokens, heads, D), dtype=x.dtype, device=x.device)
+        ot, oh = heads * D, D
+        if out.numel() == 0:
+            return out
+    # the stride of an axis of one counts for nothing
+    if tokens == 1:
+        st = ot = heads * D
+    if heads == 1:
+        sh = oh = D
+    check(lib.i4tc_rope(x.data_ptr(), _DTYPES[x.dtype], tokens, heads, D, R, st, sh, positions.data_ptr(), positions.dtype == torch.int64,
+                        freqs.data_ptr(), interleaved, scale, inverse, out.data_ptr(), ot, oh, _dev(x), _stream(x)), who)
+    return out
+
+
+def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, interleaved: bool = False, scale: float = 1.0,
+         inverse: bool = False) -> torch.Tensor:
+    """Rotary embedding of ``x`` [tokens, heads, D] (bf16 / fp16, any strides) at ``positions`` [tokens] (int32 / int64): the first
+    ``2 * len(freqs)`` elements of every head turn by ``position * freqs`` (float64, of ``rope_frequencies``) and are multiplied by
+    ``scale``, the rest is copied.  Pairs are ``(i, i + R/2)``, or ``(2i, 2i + 1)`` with ``interleaved``.  ``inverse`` turns back: it moves
+    keys to other positions, and is the gradient of ``rope``.  Angles are exact at any position; one rounding.  Returns a new
+    contiguous tensor."""
+    return _rope(x, positions, freqs, interleaved, scale, inverse, False, "rope")
+
+
+def rope_(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, interleaved: bool = False, scale: float = 1.0,
+          inverse: bool = False) -> torch.Tensor:
+    """``rope`` in place, for instance on the query and key heads of a fused QKV buffer (``qkv.view(tokens, -1, D)[:, :heads]``)."""
+    return _rope(x, positions, freqs, interleaved, scale, inverse, True, "rope_")
+
+
+_ATTENTION_ARGS = struct.Struct("@10P21qd")
+_APPEND_ARGS = struct.Struct("@8P16q")
+
+
+def _cache_pair(k_cache, v_cache, block_table, lengths, k, v):
+    """Checks of a paged cache and the new rows beside it; (k, v) with the same strides."""
+    _half_input(k, "k", 4)
+    _half_input(v, "v", 4)
+    _half_input(k_cache, "k_cache", 4)
+    _half_input(v_cache, "v_cache", 4)
+    _require(k.shape == v.shape, "k and v must have the same shape")
+    _require(k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride(), "k_cache and v_cache must have the same shape and strides")
+    _require(k.dtype == v.dtype == k_cache.dtype == v_cache.dtype, "keys, values and cache must have the same dtype")
+    _require(k_cache.shape[2:] == k.shape[2:], "k_cache must be [pages, page_size, kv_heads, D] with the new keys' kv_heads and D")
+    _require(k_cache.shape[1] > 0, "a page must hold at least one token")
+    _require(k_cache.stride(3) == 1 or k.shape[3] <= 1, "elements of a cached head must be contiguous")
+    B = k.shape[0]
+    _require(block_table.dtype == torch.int32 and block_table.dim() == 2 and block_table.shape[0] == B, "block_table must be int32 [batch, pages of a sequence]")
+    _require(lengths.dtype == torch.int32 and lengths.dim() == 1 and lengths.shape[0] == B, "lengths must be int32 [batch]")
+    dev = k.device
+    _require(v.device == dev and k_cache.device == dev and v_cache.device == dev and block_table.device == dev and lengths.device == dev,
+             "all tensors must be on the same device")
+    if k.stride() != v.stride() or k.stride(3) != 1:
+        k, v = k.contiguous(), v.contiguous()
+    return k, v, block_table if block_table.stride(1) == 1 or block_table.shape[1] <= 1 else block_table.contiguous(), lengths.contiguous()
+
+
+def kv_cache_append_(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
+                     lengths: torch.Tensor, select: torch.Tensor | None = None, counts: torch.Tensor | None = None) -> None:
+    """Writes new keys and values [B, T, kv_heads, D] into a paged cache [pages, page_size, kv_heads, D] (keys and values each, same
+    strides): row ``i < counts[b]`` (all T without ``counts``) becomes token ``lengths[b] + i`` of its sequence, in page
+    ``block_table[b, token // page_size]``, and comes from new row ``select[b, i]`` (``i`` without ``select``): a prompt, or the accepted path
+    of a tree of drafts.  All index tensors int32.  ``lengths`` stay as they are.  Counts, rows, tokens and pages out of range
+    write nothing and are raised by ``check_status``."""
+    k, v, block_table, lengths = _cache_pair(k_cache, v_cache, block_table, lengths, k, v)
+    B, T, H, D = k.shape
+    if counts is not None:
+        _require(counts.dtype == torch.int32 and counts.dim() == 1 and counts.shape[0] == B and counts.device == k.device, "counts must be int32 [batch]")
+        counts = counts.contiguous()
+    if select is not None:
+        _require(select.dtype == torch.int32 and select.dim() == 2 and select.shape[0] == B and select.device == k.device, "select must be int32 [batch, new rows]")
+        _require(select.shape[1] >= T, "select must have as many columns as there are new rows")
+        if select.stride(1) != 1:
+            select = select.contiguous()
+    new, cache = k.stride(), k_cache.stride()
+    args = _APPEND_ARGS.pack(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
+                             0 if counts is None else counts.data_ptr(), 0 if select is None else select.data_ptr(),
+                             2, B, T, H, D, k_cache.shape[0], k_cache.shape[1], block_table.shape[1], new[0], new[1], new[2], cache[0], cache[1],
+                             cache[2], block_table.stride(0), 0 if select is None else select.stride(0))
+    check(lib.i4tc_kv_append(args, _dev(k), _stream(k)), "kv_cache_append_")
+
+
+def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                   block_table: torch.Tensor, lengths: torch.Tensor, tree_mask: torch.Tensor | None = None,
+                   scale: float | None = None) -> torch.Tensor:
+    """Attention of a few new tokens (up to 64: one, a chain, or a tree of drafts) over the cache of their sequence and one another.
+
+    ``q`` [B, T, heads, D], ``k`` and ``v`` [B, T, kv_heads, D] are the new tokens' (any strides; not yet in the cache), ``heads`` a multiple of
+    ``kv_heads``, D a multiple of 8 up to 128, bf16 / fp16.  The cache is that of ``kv_cache_append_``; token t sees its sequence's
+    ``lengths[b]`` cached tokens and the new tokens j with ``tree_mask[b, t, j]`` (bool [B, T, T] or [T, T]; without one ``j <= t``).
+    A token that sees nothing gives zeros, and what a token does not see has no part in its result, infinities and NaN
+    included.  ``scale`` defaults to D ** -0.5.  Scores, weights' sums and results are held in fp32; a weight is rounded to the
+    values' type before it multiplies them, as the tensor cores take it, and summed as rounded.  Returns [B, T, heads, D].  Pages
+    and lengths out of range are raised by ``check_status``."""
+    _half_input(q, "q", 4)
+    k, v, block_table, lengths = _cache_pair(k_cache, v_cache, block_table, lengths, k, v)
+    B, T, H, D = q.shape
+    Hk = k.shape[2]
+    _require(q.dtype == k.dtype and q.device == k.device, "queries must have the keys' dtype and device")
+    _require(k.shape == (B, T, Hk, D), "q must be [B, T, heads, D] and k [B, T, kv_heads, D]")
+    _require(T <= 64, "at most 64 new tokens a sequence")
+    _require(D % 8 == 0 and 0 < D <= 128, "heads must have a multiple of 8 and at most 128 elements")
+    _require(Hk > 0 and H % Hk == 0, "heads must be a multiple of kv_heads")
+    out = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
+    if out.numel() == 0:
+        return out
+    mask_ptr = mask_batch = 0
+    if tree_mask is not None:
+        _require(tree_mask.dtype == torch.bool and tree_mask.device == q.device, "tree_mask must be bool, on the queries' device")
+        _require(tree_mask.shape == (B, T, T) or tree_mask.shape == (T, T), "tree_mask must be [B, T, T] or [T, T]")
+        tree_mask = tree_mask.contiguous()
+        mask_ptr, mask_batch = tree_mask.data_ptr(), T * T if tree_mask.dim() == 3 else 0
+    sq = q.stride()
+    if sq[3] != 1 or sq[0] % 2 or sq[1] % 2 or sq[2] % 2 or q.data_ptr() % 4:
+        q = q.clone(memory_format=torch.contiguous_format)
+        sq = q.stride()
+    new, cache = k.stride(), k_cache.stride()
+    if new[0] % 8 or new[1] % 8 or new[2] % 8 or k.data_ptr() % 16 or v.data_ptr() % 16:
+        k, v = (t.clone(memory_format=torch.contiguous_format) for t in (k, v))
+        new = k.stride()
+    _require(k_cache.data_ptr() % 16 == 0 and v_cache.data_ptr() % 16 == 0 and cache[0] % 8 == 0 and cache[1] % 8 == 0 and cache[2] % 8 == 0,
+             "cached heads must be 16-byte aligned")
+    dev, width, page = _dev(q), block_table.shape[1], k_cache.shape[1]
+    nbytes = lib.i4tc_tree_attention_scratch_bytes(B, T, H, Hk, D, width * page, dev)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    args = _ATTENTION_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
+                                lengths.data_ptr(), mask_ptr, out.data_ptr(), scratch.data_ptr(), nbytes, _DTYPES[q.dtype], B, T, H, Hk, D,
+                                k_cache.shape[0], page, width, sq[0], sq[1], sq[2], new[0], new[1], new[2], cache[0], cache[1], cache[2],
+                                block_table.stride(0), mask_batch, D ** -0.5 if scale is None else scale)
+    check(lib.i4tc_tree_attention(args, dev, _stream(q)), "tree_attention")
+    return out
+
+
 def set_tuning(tile_n: int = 0, swap: int = -1) -> None:
     """Force the GEMM tile width / operand orientation (tests); ``set_tuning()`` restores automatic."""
     check(lib.i4tc_set_tuning(tile_n, swap), "set_tuning")
@@ -558,6 +786,7 @@ def workspace_bytes(device=None, stream=None) -> int:
 
 
 def check_status(device=None) -> None:
-    """Raise if any kernel gave up on a bounded wait since the last call (synchronises the stream)."""
+    """Raise if any kernel gave up on a bounded wait, or met a length, page or index out of range, since the last call
+    (synchronises the stream)."""
     dev = torch.cuda.current_device() if device is None else torch.device(device).index
     check(lib.i4tc_check_status(dev, torch.cuda.current_stream(dev).cuda_stream), "check_status")

@@ -34,7 +34,7 @@ extern "C" {
 #define I4TC_EALIGN (-2)      /* pointer or stride not aligned as required       */
 #define I4TC_EUNSUPPORTED (-3)/* combination not implemented                     */
 #define I4TC_EDEVICE (-4)     /* device is not compute capability 10.x           */
-#define I4TC_EKERNEL (-5)     /* a kernel reported a bounded-wait timeout        */
+#define I4TC_EKERNEL (-5)     /* a kernel reported a bounded-wait timeout, or an index out of range */
 #define I4TC_EWORKSPACE (-6)  /* the split-K workspace could not be grown        */
 
 /* element types of floating-point inputs / outputs */
@@ -409,8 +409,62 @@ int i4tc_qk_norm_rope(void* qkv, int64_t tokens, int64_t ld, int64_t q_heads, in
                       const void* q_weight, const void* k_weight, const void* cos_table, const void* sin_table, float eps,
                       int device, void* stream);
 
-/* Polls the device-side status word written by bounded waits; 0 if no kernel timed out since
- * the last call, else I4TC_EKERNEL.  Synchronises `stream`. */
+/* ---- decoding: a few tokens a sequence over 4-bit weights and a paged cache ---- */
+
+/* out [M, N] = x [M, K] . W^T of bf16 / fp16 activations (row stride ldx elements) and int4 weights in either layout (codes
+ * [G, rows, 64] with scales [G, rows]; per_channel: [rows, K/2] with [rows]), without quantising the activations:
+ * exact products, fp32 sums, one rounding.  gated: W has 2 N rows and out = silu(x . W[0, N)^T) * (x . W[N, 2 N)^T).
+ * Made for up to 32 tokens; more read the weights once for every 32. */
+int i4tc_w4a16_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* w, const float* w_scale,
+                      int per_channel, int gated, void* out, int64_t N, int device, void* stream);
+
+/* Rotary embedding of the first R of D elements of x [tokens, heads, D] (bf16 / fp16, strides in elements, elements of a head
+ * contiguous) at positions [tokens] (int32, or int64 with long_positions): a pair (a, b) becomes
+ * scale * (a cos - b sin, b cos + a sin) with the angle position * freqs[i] (float64 [R/2], radians a position), minus the angle with
+ * inverse.  Pairs are (i, i + R/2), interleaved: (2i, 2i + 1).  Elements behind R are copied.  out may be x (same strides). */
+int i4tc_rope(const void* x, int dtype, int64_t tokens, int64_t heads, int64_t D, int64_t R, int64_t x_token, int64_t x_head,
+              const void* positions, int long_positions, const double* freqs, int interleaved, float scale, int inverse,
+              void* out, int64_t out_token, int64_t out_head, int device, void* stream);
+
+/* Attention of `tokens` new tokens of every sequence over its cache and over one another:
+ *   q [batch, tokens, heads, D], k and v [batch, tokens, kv_heads, D], out [batch, tokens, heads, D] contiguous (bf16 / fp16);
+ *   k_cache, v_cache [pages, page_size, kv_heads, D]; block_table [batch, table_width] and lengths [batch] int32: token j < lengths[b]
+ *   is row j % page_size of page block_table[b, j / page_size].
+ * New token t sees the whole cache of its sequence and the new tokens j with mask[b, t, j] != 0 (bytes [tokens, tokens], mask_batch
+ * apart, 0 for one that all share; NULL: j <= t).  A token that sees nothing gives zeros.  Strides in elements, multiples of 8
+ * (queries: of 2); k and v share theirs, the caches share theirs.  At most 64 new tokens, D a multiple of 8 up to 128.  Lengths
+ * beyond the table and pages out of range set bit 2 of the status word (i4tc_check_status), and read nothing.
+ * scratch: i4tc_tree_attention_scratch_bytes with most_length = table_width * page_size; free again when the call's
+ * work on its stream is done. */
+typedef struct {
+  const void *q, *k, *v, *k_cache, *v_cache;
+  const int32_t *block_table, *lengths;
+  const uint8_t* mask;
+  void* out;
+  void* scratch;
+  int64_t scratch_bytes, dtype, batch, tokens, heads, kv_heads, head_dim, pages, page_size, table_width;
+  int64_t q_batch, q_token, q_head, new_batch, new_token, new_head, page_stride, slot_stride, head_stride, table_stride, mask_batch;
+  double scale;
+} i4tc_tree_attention_args;
+int64_t i4tc_tree_attention_scratch_bytes(int64_t batch, int64_t tokens, int64_t heads, int64_t kv_heads, int64_t D,
+                                          int64_t most_length, int device);
+int i4tc_tree_attention(const i4tc_tree_attention_args* args, int device, void* stream);
+
+/* Rows i < counts[b] (NULL: all `tokens`) of every sequence go into its cache as tokens lengths[b] + i, taken from new row
+ * select[b, i] (int32, select_stride apart; NULL: i) of k and v [batch, tokens, kv_heads, D].  Cache, table and strides as above, of any
+ * alignment.  Nothing else of the cache is written, and lengths stay as they are.  Counts, indices, tokens beyond the table
+ * and pages out of range set bit 2 of the status word, and write nothing. */
+typedef struct {
+  const void *k, *v;
+  void *k_cache, *v_cache;
+  const int32_t *block_table, *lengths, *counts, *select;
+  int64_t element_bytes, batch, tokens, kv_heads, head_dim, pages, page_size, table_width;
+  int64_t new_batch, new_token, new_head, page_stride, slot_stride, head_stride, table_stride, select_stride;
+} i4tc_kv_append_args;
+int i4tc_kv_append(const i4tc_kv_append_args* args, int device, void* stream);
+
+/* Polls the device-side status word written by bounded waits and range checks; 0 if no kernel timed out or
+ * met an index out of range since the last call, else I4TC_EKERNEL.  Synchronises `stream`. */
 int i4tc_check_status(int device, void* stream);
 
 #ifdef __cplusplus
