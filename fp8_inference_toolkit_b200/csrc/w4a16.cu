@@ -3,21 +3,34 @@
 //   y[m, n] = sum_g s[g, n] * sum_{k in group g} x[m, k] * c[n, k]        (one scale a row: s[n] * sum_k ...)
 //   gated:    h[m, n] = silu(y[m, n]) * y[m, N + n]                       (weight rows [0, N) gate, [N, 2 N) up)
 //
-// Bound: the weights' bytes, read once.  Half a byte gives 2 M operations, so tensor instructions fed from registers are fast
-// enough (mma.sync; a tcgen05 tile would be padding at these M and would want the expanded codes in shared memory first), and what
-// counts is the bytes in flight.  A warp takes 16 MT weight rows and one 128-code unit a step: a unit's 16 rows are
-// 1 KB in one piece, a lane holds 32 codes of two rows as two 16-byte loads, DEPTH units are on their way before the first is
-// used, and the stream runs on over the block's row tiles without a break.  The tokens stay in shared memory, laid out once as
-// the instruction's operand.
+// Bound: the weights' bytes, read once; then the instructions that a code costs.  Half a byte gives 2 M operations, so tensor
+// instructions fed from registers are fast enough (mma.sync; a tcgen05 tile would be padding at these M and would want the expanded
+// codes in shared memory first): an m16n8k16 takes a scheduler 8 cycles, and masking instructions run beside it.
 //
-// Codes become exact 16-bit numbers without a conversion: a nibble, its top bit flipped, is or-ed (in one instruction with the
-// mask) under the exponent of 128 (bf16) or 1024 (fp16), and one subtraction takes that off again.  The k order inside an
-// instruction is free as long as both operands agree: a word's nibbles come out as pairs (i, i + 4), and the tokens are
-// laid out in these pairs.  Products of a code and a 16-bit number are exact in fp32 and all sums are fp32; the result is rounded once.
+// A block (sixteen warps, one an SM) takes a contiguous range of 16-row tiles, so that every SM has the same share whatever N is.
+// Its warps take the tiles in turn, split K, or both.  A step is one tile's 128 codes of K (1 KB) and their scales, which a lane
+// copies for itself into a ring of the warp's, up to eight steps ahead, by cp.async: no registers and no barrier, and no waiting on
+// loads issued later (with the ring in registers the six scoreboards of a warp were shared between its steps: 19.5 us instead
+// of 14.9 for the gated [1, 4096] x [24576, 4096]; bulk copies on mbarriers cost 80 instructions a step).
 //
-// The eight warps of a block take every eighth unit and are added in ascending order through shared memory.  Where the tokens do
-// not fit a block's shared memory, a cluster of 2 to 8 blocks splits K, and its ranks are added in order through
-// distributed shared memory: no workspace, and the same bits in every run.
+// Codes become operands by one masking instruction each (and a shift for every second pair): a nibble in the low bits of a 16-bit
+// word, its top bit flipped, is the fp16 subnormal (code + 8) * 2^-24, one bit group further up (code + 8) * 2^-20.  The
+// tokens meet them as fp16 too: the 128 numbers of a step are scaled by the power of two that brings the largest to 2^15 (a
+// sixteenth of that where they meet the upper nibbles), which is exact for all that are not 2^28 times smaller, and 8 times their sum
+// comes off the result.  Products are exact and sums fp32 as they would be with codes and tokens themselves; the +8 makes their terms
+// three times larger.  Where a number would not stay exact, or is infinite or none, the block takes the plain way: codes as numbers
+// of the tokens' type (128 + 8 or 1024 + 8 taken off by a subtraction), tokens as they are.  So do more than eight tokens, for
+// which the tensor instructions bound the walk.
+//
+// The k order inside an instruction is free as long as both operands agree: a word's nibbles come out as pairs (i, i + 4), and the
+// tokens are laid out in these pairs, once, in shared memory.
+//
+// A cluster of up to eight blocks shares the same rows and splits K, where the tokens of long K would not fit a block, or where
+// laying them out in every block costs more than adding up; its partial sums are added in ascending order through distributed
+// shared memory: no workspace, no second launch, and the same bits in every run.
+//
+// Measured (device time, weights from HBM, bf16, per-group scales): [1, 4096] x [6144, 4096] 5.7 us, [16, 12288] x [4096, 12288]
+// 18.1, gated [1, 4096] x [24576, 4096] 14.9 (3.6 TB/s), [16, ...] 22.7, [32, ...] 42.
 #include "common.cuh"
 #include "ptx.cuh"
 #include <type_traits>
@@ -26,9 +39,10 @@ namespace i4tc {
 
 namespace {
 
-constexpr int kWarps = 8, kThreads = kWarps * 32;
-constexpr int kMostTokens = 32;                  // of a launch's grid row; more tokens read the weights again
-constexpr size_t kMostSmem = 220 * 1024;
+constexpr int kWarps = 16, kThreads = kWarps * 32;
+constexpr int kMostTokens = 32;                     // of a launch's grid row; more tokens read the weights again
+constexpr size_t kMostSmem = 224 * 1024;
+constexpr int kStep = 16 * 64 + 16 * 4;             // bytes of a step: sixteen rows of 128 codes, and their scales
 
 struct W4A16Params {
   const void* x;
@@ -41,239 +55,358 @@ struct W4A16Params {
   int units;            // ceil(K / 128)
   int units_each;       // of a cluster rank
   int ranks;            // blocks of a cluster
-  int tiles;            // of 16 MT weight rows (gated: 16 columns)
+  int tiles;            // of sixteen weight rows
+  int tile_warps;       // warps of a block that take its tiles in turn; the others split the block's K
+  int steps;            // units of a warp, at most
   int most_tokens;      // of a grid row
 };
 
-template <typename T>
-__device__ __forceinline__ uint32_t codes_pair(uint32_t w) {   // nibbles 0 and 4 of w as two numbers of type T
-  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-    const uint32_t u = (w & 0x000F000Fu) ^ 0x43084308u;        // 128 + (code + 8)
-    const uint32_t o = 0x43084308u;                             // 136
-    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&o));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  } else {
-    const uint32_t u = (w & 0x000F000Fu) ^ 0x64086408u;        // 1024 + (code + 8)
-    const uint32_t o = 0x64086408u;                             // 1032
-    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&o));
-    return *reinterpret_cast<const uint32_t*>(&r);
-  }
-}
-
-template <typename T>
+// c = a b, or with ADD c += a b.
+template <typename T, bool ADD>
 __device__ __forceinline__ void mma16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  const float z[4] = {ADD ? c[0] : 0.f, ADD ? c[1] : 0.f, ADD ? c[2] : 0.f, ADD ? c[3] : 0.f};
   if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(z[0]), "f"(z[1]), "f"(z[2]), "f"(z[3]));
   } else {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
-                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %11, %12, %13};"
+                 : "=f"(c[0]), "=f"(c[1]), "=f"(c[2]), "=f"(c[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(z[0]), "f"(z[1]), "f"(z[2]), "f"(z[3]));
   }
 }
 
-__device__ __forceinline__ uint4 load_stream(const uint8_t* p) {   // read once: not kept in L1
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+// 16 bytes global -> shared without registers in between; where not valid, nothing is read and zeros are written.
+__device__ __forceinline__ void copy_16(uint32_t dst, const uint8_t* src, bool valid) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16u : 0u) : "memory");
+}
+// (w & MASK) ^ flip in one instruction: one immediate operand, the other in a register that the compiler does not see through.
+template <uint32_t MASK>
+__device__ __forceinline__ uint32_t mask_flip(uint32_t w, uint32_t flip) {
+  uint32_t u;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6A;" : "=r"(u) : "r"(w), "n"(MASK), "r"(flip));
+  return u;
+}
+template <uint32_t V>
+__device__ __forceinline__ uint32_t opaque() {
+  uint32_t v;
+  asm volatile("mov.u32 %0, %1;" : "=r"(v) : "n"(V));
   return v;
+}
+
+// Nibbles 0 and 4 of w as two numbers of type T.
+template <typename T>
+__device__ __forceinline__ uint32_t codes_pair(uint32_t w, uint32_t bias) {
+  const uint32_t u = mask_flip<0x000F000Fu>(w, bias);
+  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
+    const __nv_bfloat162 r = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&u), *reinterpret_cast<const __nv_bfloat162*>(&bias));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  } else {
+    const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&bias));
+    return *reinterpret_cast<const uint32_t*>(&r);
+  }
 }
 
 __device__ __forceinline__ void store_as(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store_as(__half* p, float v) { *p = __float2half_rn(v); }
 
-// Floats of one warp's partial sums: rows padded so that the lanes of a fragment hit different banks.
-__host__ __device__ constexpr int red_row(int mt) { return 16 * mt + 4; }
-__host__ __device__ constexpr size_t w4a16_smem(int tokens, int units_each, int mt, int ranks) {
-  return (size_t)units_each * tokens * 256                                // the tokens
-         + (size_t)kWarps * tokens * red_row(mt) * 4                      // partial sums of the warps
-         + (size_t)2 * (ranks - 1) * tokens * 16 * mt * 4;                // and of the other ranks, two tiles' worth
+constexpr int token_tiles(int tokens, bool small) { return small || tokens > 16 ? 4 : tokens > 8 ? 2 : 1; }
+constexpr int ring_depth(int token_tiles) { return token_tiles == 1 ? 8 : 4; }
+constexpr size_t w4a16_smem(int tokens, bool small, int units_each, int block_tiles, int k_warps) {
+  return (size_t)units_each * tokens * 256                              // the tokens
+         + (size_t)units_each * token_tiles(tokens, small) * 64         // factor and offset of each in a step
+         + (size_t)block_tiles * k_warps * tokens * 64                  // partial sums
+         + (size_t)kWarps * ring_depth(token_tiles(tokens, small)) * kStep;   // rings
 }
 
-// NT: 8-token tiles.  MT: 16-row tiles of a warp (gated: one of gate rows, one of up rows).  ROWMAJOR: codes [rows, K / 2] and one
-// scale a row, else [units, rows, 64] and a scale for each unit.
-template <typename T, int NT, int MT, bool GATED, bool ROWMAJOR, int DEPTH>
-__global__ void __launch_bounds__(kThreads) w4a16_kernel(const W4A16Params p) {
-  static_assert(!GATED || MT == 2, "gate and up");
+template <typename T> struct Bits;   // of the tokens' type: exponent's place, bias and highest value
+template <> struct Bits<__nv_bfloat16> { static constexpr int kShift = 7, kBias = 127, kTop = 255; };
+template <> struct Bits<__half> { static constexpr int kShift = 10, kBias = 15, kTop = 31; };
+
+// NT: 8-token tiles.  GATED: a tile's sixteen rows are eight columns' gate rows and then their up rows.  ROWMAJOR: codes [rows, K / 2]
+// and one scale a row, else [units, rows, 64] and a scale for each unit.  SMALL: fewer columns than a tile has.
+template <typename T, int NT, bool GATED, bool ROWMAJOR, bool SMALL>
+__global__ void __launch_bounds__(kThreads, 1) w4a16_kernel(const W4A16Params p) {
+  constexpr int COLS = GATED ? 8 : 16, DEPTH = ring_depth(NT);
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int g = lane >> 2, t = lane & 3;
   const int rank = blockIdx.y, u0 = rank * p.units_each;
   const int units = min(p.units_each, p.units - u0);
   const int m0 = blockIdx.z * p.most_tokens, M = min(p.most_tokens, p.M - m0);
-  uint4* xs = reinterpret_cast<uint4*>(smem);                             // [unit][word][token][t]
-  float* red = reinterpret_cast<float*>(smem + (size_t)p.units_each * M * 256);   // [warp][token][row]
-  float* other = red + kWarps * M * red_row(MT);                          // [parity][rank - 1][token][row]
+  const int tile0 = (int)((long long)blockIdx.x * p.tiles / gridDim.x), ntiles = (int)((long long)(blockIdx.x + 1) * p.tiles / gridDim.x) - tile0;
+  const int wn = warp % p.tile_warps, wk = warp / p.tile_warps, k_warps = kWarps / p.tile_warps;
+  const int first = min(units, wk * p.steps), mine = min(units, first + p.steps) - first;   // of the block's units, this warp's
+  uint4* xs = reinterpret_cast<uint4*>(smem);                             // [unit][token][word][t], words of odd tokens swapped in pairs
+  float2* ab = reinterpret_cast<float2*>(xs + (size_t)p.units_each * M * 16);   // [unit][8 NT]: factor of a token's sums, and what comes off
+  uint8_t* rings = reinterpret_cast<uint8_t*>(ab + p.units_each * 8 * NT);      // [warp][slot][16 rows of codes, 16 scales]
+  float* part = reinterpret_cast<float*>(rings + kWarps * DEPTH * kStep); // [tile][k warp][token][16]
+  const uint32_t ring = ptx::smem_u32(rings) + warp * DEPTH * kStep, ring_lane = ring + lane * 16;
 
   const T* x = pdl_wait(static_cast<const T*>(p.x));
   const uint8_t* w = p.w;
   const float* sw = p.sw;
   pdl_fresh(w); pdl_fresh(sw);
+  pdl_trigger();
 
-  const int steps = (units + kWarps - 1) / kWarps;                        // of a row tile; the same for every warp
-  uint4 ring[DEPTH][MT][2];
-  float scale[DEPTH][MT][2];
-  int f_tile = blockIdx.x, f_step = 0;                                    // where the loads are
-  // Rows behind the last read the last row (their sums go nowhere); units behind the last are zero codes.
-  auto fetch = [&](uint4 (&v)[MT][2], float (&s)[MT][2]) {
-    const int u = f_step * kWarps + warp;
-    if (f_tile < p.tiles && u < units) {
+  // The last tile begins early enough to be full: its first columns are the tile's before it, too, with the same bits.
+  auto first_column = [&](int tile) -> long long { return SMALL ? 0 : min(tile * COLS, p.N - COLS); };
+  // Row r of a tile, counted from its first column: rows behind the last read the last (their sums go nowhere).
+  auto row_of = [&](int r) -> long long {
+    const int c = GATED ? r & 7 : r;
+    return (SMALL ? min(c, p.N - 1) : c) + (GATED && r >= 8 ? (long long)p.N : 0);
+  };
+  const int total = ntiles > wn && mine > 0 ? (ntiles - wn + p.tile_warps - 1) / p.tile_warps * mine : 0;   // steps of this warp
+  // Where its copies are: lane (g, t) copies 32 codes each of rows g and 8 + g, for itself, and one of sixteen lanes a scale.
+  const long long row_bytes = ROWMAJOR ? p.K / 2 : 64, unit_step = ROWMAJOR ? 64 : (long long)p.rows * 64;
+  const uint8_t* const base_w = w + (ROWMAJOR ? (long long)(u0 + first) * 64 : (long long)(u0 + first) * p.rows * 64) + row_of(g) * row_bytes + t * 16;
+  const float* const base_s = sw + (long long)(u0 + first) * p.rows + row_of(lane & 15);
+  const long long second = row_of(8 + g) - row_of(g);
+  const int lane_units = ROWMAJOR ? (p.K - (u0 + first) * 128 - t * 32 + 127) / 128 : 0;   // row-major: the last unit may be half
+  int a_tile = tile0 + wn, a_u = 0;
+  const uint8_t* a_w;
+  const float* a_s;
+  auto aim = [&]() {
+    const long long row = first_column(a_tile);
+    a_w = base_w + row * row_bytes;
+    a_s = base_s + row;
+  };
+  auto fetch = [&](int slot) {
+    const uint32_t to = ring_lane + slot * kStep;
+    const bool in = !ROWMAJOR || a_u < lane_units;
+    copy_16(to, in ? a_w : w, in);
+    copy_16(to + 512, in ? a_w + second * row_bytes : w, in);
+    if constexpr (!ROWMAJOR) {
+      if (lane < 16) ptx::cp_async_4_zfill(ring + slot * kStep + 1024 + lane * 4, a_s, true);
+      a_s += p.rows;
+    }
+    a_w += unit_step;
+    if (++a_u == mine) {
+      a_u = 0;
+      a_tile += p.tile_warps;
+      aim();                                                              // (an address only: behind the last tile nothing is read)
+    }
+  };
+  aim();
 #pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
+  for (int d = 0; d < DEPTH; ++d) {
+    if (d < total) fetch(d);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+
+  // The tokens, as the operand of the instruction: 16 bytes = eight numbers of one token in pairs (i, i + 4).  Sixteen lanes have a token's
+  // numbers of a unit.  PLAIN: as they are.  Returns whether a number would not stay exact.
+  auto lay_out = [&](auto plain) {
+    constexpr bool PLAIN = decltype(plain)::value;
+    bool lost = false;
+    const int c = threadIdx.x & 15;                                       // 16 bytes of the 256
+    int u = threadIdx.x >> 4, m = 0;
+    while (u >= units) { u -= units; ++m; }
+#pragma unroll 2
+    for (int i0 = 0; i0 < units * M; i0 += kThreads / 16) {
+      const int k = (u0 + u) * 128 + c * 8;
+      const bool in = m < M;
+      uint4 v = make_uint4(0u, 0u, 0u, 0u);
+      if (in && k < p.K) v = __ldg(reinterpret_cast<const uint4*>(x + (long long)(m0 + m) * p.ldx + k));
+      uint4 r = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+      if constexpr (!PLAIN) {
+        uint32_t top = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
+        top = max(top & 0xFFFFu, top >> 16);
+        uint32_t* pair = &r.x;
+        float lo[4], hi[4], sum = 0.f;
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          int r = (GATED ? f_tile * 16 : f_tile * 16 * MT + 16 * mt) + g + 8 * h;
-          r = min(r, p.N - 1) + (GATED && mt == 1 ? p.N : 0);
-          if constexpr (ROWMAJOR) {
-            const int k = (u0 + u) * 128 + t * 32;
-            v[mt][h] = make_uint4(0u, 0u, 0u, 0u);
-            if (k < p.K) v[mt][h] = load_stream(w + (long long)r * (p.K / 2) + k / 2);
-          } else {
-            const long long at = (long long)(u0 + u) * p.rows + r;
-            v[mt][h] = load_stream(w + at * 64 + t * 16);
-            s[mt][h] = __ldg(sw + at);
+        for (int j = 0; j < 4; ++j) {
+          lo[j] = to_f32(reinterpret_cast<const T*>(pair + j)[0]);
+          hi[j] = to_f32(reinterpret_cast<const T*>(pair + j)[1]);
+          sum += lo[j] + hi[j];
+        }
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) {
+          top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+          sum += __shfl_xor_sync(0xffffffffu, sum, o);
+        }
+        const int e = top >> Bits<T>::kShift;
+        const int up = min(15 + Bits<T>::kBias - max(e, 1), 120);         // times 2^up
+        lost |= e == Bits<T>::kTop || up < -100;
+        const float f = __uint_as_float((uint32_t)(127 + up) << 23), back = __uint_as_float((uint32_t)(127 - up) << 23);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float fj = j & 1 ? f * 0.0625f : f, bj = j & 1 ? back * 16.0f : back;
+          const __half2 h = __floats2half2_rn(lo[j] * fj, hi[j] * fj);
+          const float2 again = __half22float2(h);
+          lost |= again.x * bj != lo[j] || again.y * bj != hi[j];
+          pair[j] = *reinterpret_cast<const uint32_t*>(&h);
+        }
+        if (in && c == 0) ab[u * 8 * NT + m] = make_float2(back * 16777216.0f, 8.0f * sum);
+      }
+      if (in) xs[(u * M + m) * 16 + ((c & 3) ^ (m & 1)) * 4 + (c >> 2)] = r;
+      u += kThreads / 16;
+      while (u >= units) { u -= units; ++m; }
+    }
+    return lost;
+  };
+  // (with more than eight tokens the scaling of all of them costs more than it saves: the tensor instructions bound the walk)
+  bool plain = true;
+  if constexpr (NT == 1) plain = __syncthreads_or(lay_out(std::false_type{}));
+  if (plain) {
+    lay_out(std::true_type{});
+    __syncthreads();
+  }
+
+  // a lane without a token of its own reads the last one: its column of the result goes nowhere
+  uint32_t b_at[NT];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int m = min(8 * nt + g, M - 1);
+    b_at[nt] = ptx::smem_u32(xs) + (m * 16 + (m & 1) * 4 + t) * 16;
+  }
+  auto walk = [&](auto plain_way) {
+    constexpr bool PLAIN = decltype(plain_way)::value;
+    // 128 + 8 in bf16 or 1024 + 8 in fp16, twice; the sign bits of the codes in either place
+    const uint32_t bias = opaque<std::is_same_v<T, __nv_bfloat16> ? 0x43084308u : 0x64086408u>();
+    const uint32_t flip_lo = opaque<0x00080008u>(), flip_hi = opaque<0x00800080u>();
+    float f[NT][4];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f[nt][i] = 0.f;
+    uint32_t b_off = first * M * 256;
+    int u = 0, tile = wn;
+    int slot = 0;
+    {
+      for (int i = 0; i < total; ++i) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+        __syncwarp();
+        {
+          const uint32_t from = ring_lane + slot * kStep;
+          const uint4 v0 = ptx::lds128(from), v1 = ptx::lds128(from + 512);
+          float s0 = 1.0f, s1 = 1.0f;
+          if constexpr (!ROWMAJOR) {
+            const uint32_t s_from = ring + slot * kStep + 1024 + g * 4;
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s0) : "r"(s_from));
+            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s1) : "r"(s_from + 32));
+          }
+          float c[NT][4];
+#pragma unroll
+          for (int q = 0; q < 4; ++q) {
+            uint32_t a[8];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              const uint4& v = h ? v1 : v0;
+              const uint32_t word = q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w;
+              if constexpr (PLAIN) {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) a[2 * k + h] = codes_pair<T>(word >> (4 * k), bias);
+              } else {
+                a[h] = mask_flip<0x000F000Fu>(word, flip_lo);
+                a[2 + h] = mask_flip<0x00F000F0u>(word, flip_hi);
+                a[4 + h] = mask_flip<0x000F000Fu>(word >> 8, flip_lo);
+                a[6 + h] = mask_flip<0x00F000F0u>(word >> 8, flip_hi);
+              }
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              const uint4 b = ptx::lds128(((b_at[nt] + b_off) ^ ((q & 1) * 64)) + (q >> 1) * 128);
+              using A = std::conditional_t<PLAIN, T, __half>;
+              if (q == 0) mma16<A, false>(c[nt], a[0], a[1], a[2], a[3], b.x, b.y);
+              else mma16<A, true>(c[nt], a[0], a[1], a[2], a[3], b.x, b.y);
+              mma16<A, true>(c[nt], a[4], a[5], a[6], a[7], b.z, b.w);
+            }
+          }
+          __syncwarp();                                                   // the slot has been read
+          if (i + DEPTH < total) fetch(slot);
+          asm volatile("cp.async.commit_group;" ::: "memory");
+          if (++slot == DEPTH) slot = 0;
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            float4 k = make_float4(1.f, 0.f, 1.f, 0.f);
+            if constexpr (!PLAIN) k = *reinterpret_cast<const float4*>(ab + ((first + u) * NT + nt) * 8 + 2 * t);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+              const float s = PLAIN ? c[nt][j] : fmaf(c[nt][j], j & 1 ? k.z : k.x, j & 1 ? -k.w : -k.y);
+              f[nt][j] = fmaf(s, j >> 1 ? s1 : s0, f[nt][j]);
+            }
+          }
+          b_off += M * 256;
+          if (++u == mine) {                                              // the tile's sums over this warp's units
+            float* to = part + (tile * k_warps + wk) * M * 16;
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                const int m = 8 * nt + 2 * t + (j & 1);
+                if (m < M) to[m * 16 + g + 8 * (j >> 1)] = f[nt][j];
+                f[nt][j] = 0.f;
+              }
+            u = 0;
+            b_off = first * M * 256;
+            tile += p.tile_warps;
           }
         }
       }
     }
-    if (++f_step == steps) { f_step = 0; f_tile += gridDim.x; }
   };
-#pragma unroll
-  for (int d = 0; d < DEPTH; ++d) fetch(ring[d], scale[d]);
-
-  // the tokens, as the operand of the instruction: 16 bytes = eight numbers of one token in pairs (i, i + 4)
-  for (int i = threadIdx.x; i < units * 16 * M; i += kThreads) {
-    const int m = i / (units * 16), c = i - m * (units * 16), k = u0 * 128 + c * 8;
-    uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (k < p.K) v = __ldg(reinterpret_cast<const uint4*>(x + (long long)(m0 + m) * p.ldx + k));
-    xs[(((c >> 4) * 4 + (c & 3)) * M + m) * 4 + ((c >> 2) & 3)] =
-        make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
+  if constexpr (NT == 1) {
+    if (!plain) walk(std::false_type{});
   }
-  if (p.ranks > 1) ptx::cluster_sync(); else __syncthreads();
+  if (plain) walk(std::true_type{});
+  __syncthreads();
 
-  float f[MT][NT][4];
-  int tile = blockIdx.x, step = 0, parity = 0;
-  auto clear = [&](float (&a)[MT][NT][4]) {
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) a[mt][nt][i] = 0.f;
+  // the warps' sums in ascending order (those that have units), then the ranks'
+  const int with_work = min(k_warps, (units + p.steps - 1) / p.steps), values = ntiles * M * COLS;
+  auto added = [&](int at) {
+    float v = part[at];
+    for (int k = 1; k < with_work; ++k) v += part[at + k * M * 16];
+    return v;
   };
-  auto multiply = [&](const uint4 (&v)[MT][2], int u, float (&c)[MT][NT][4]) {
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      uint4 b[NT];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        b[nt] = make_uint4(0u, 0u, 0u, 0u);
-        if (8 * nt + g < M) b[nt] = xs[((u * 4 + q) * M + 8 * nt + g) * 4 + t];
-      }
-#pragma unroll
-      for (int mt = 0; mt < MT; ++mt) {
-        const uint32_t a = q == 0 ? v[mt][0].x : q == 1 ? v[mt][0].y : q == 2 ? v[mt][0].z : v[mt][0].w;
-        const uint32_t e = q == 0 ? v[mt][1].x : q == 1 ? v[mt][1].y : q == 2 ? v[mt][1].z : v[mt][1].w;
-        const uint32_t a0 = codes_pair<T>(a), a1 = codes_pair<T>(a >> 4), a2 = codes_pair<T>(a >> 8), a3 = codes_pair<T>(a >> 12);
-        const uint32_t e0 = codes_pair<T>(e), e1 = codes_pair<T>(e >> 4), e2 = codes_pair<T>(e >> 8), e3 = codes_pair<T>(e >> 12);
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          mma16<T>(c[mt][nt], a0, e0, a1, e1, b[nt].x, b[nt].y);
-          mma16<T>(c[mt][nt], a2, e2, a3, e3, b[nt].z, b[nt].w);
-        }
-      }
+  auto finish = [&](int tile, int m, int r, float v, float up) {
+    const long long n = first_column(tile0 + tile) + r;
+    if (SMALL && n >= p.N) return;
+    if constexpr (ROWMAJOR) v *= __ldg(sw + n);
+    if constexpr (GATED) {
+      if constexpr (ROWMAJOR) up *= __ldg(sw + p.N + n);
+      v = v / (1.0f + expf(-v)) * up;
     }
+    store_as(static_cast<T*>(p.out) + (long long)(m0 + m) * p.N + n, v);
   };
-  // The tile's sums, warp by warp and rank by rank in ascending order; every thread of the block (of the cluster) comes here.
-  auto finish = [&]() {
-    float* mine = red + warp * M * red_row(MT);
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const int m = 8 * nt + 2 * t + (i & 1);
-          if (m < M) mine[m * red_row(MT) + 16 * mt + g + 8 * (i >> 1)] = f[mt][nt][i];
-        }
-    __syncthreads();
-    auto sum = [&](int m, int r) {
-      float v = 0.f;
-#pragma unroll
-      for (int k = 0; k < kWarps; ++k) v += red[(k * M + m) * red_row(MT) + r];
-      return v;
-    };
-    const int values = M * 16 * MT;
-    if (p.ranks > 1) {
-      if (rank > 0) {
-        const uint32_t to = ptx::mapa_shared(ptx::smem_u32(other + (parity * (p.ranks - 1) + rank - 1) * values), 0);
-        for (int i = threadIdx.x; i < values; i += kThreads) {
-          const int m = i / (16 * MT), r = i - m * (16 * MT);
-          asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + 4u * i), "f"(sum(m, r)) : "memory");
-        }
-      }
-      ptx::cluster_sync();
+  if (p.ranks == 1) {
+    for (int i = threadIdx.x; i < values; i += kThreads) {
+      const int r = i % COLS, q = i / COLS, tile = q / M, m = q - tile * M, at = (tile * k_warps * M + m) * 16 + r;
+      finish(tile, m, r, added(at), GATED ? added(at + 8) : 0.f);
     }
-    if (rank == 0) {
-      const float* more = other + parity * (p.ranks - 1) * values;
-      auto total = [&](int m, int r) {
-        float v = sum(m, r);
-        for (int k = 0; k + 1 < p.ranks; ++k) v += more[(k * M + m) * (16 * MT) + r];
-        return v;
-      };
-      constexpr int COLS = GATED ? 16 : 16 * MT;
-      for (int i = threadIdx.x; i < M * COLS; i += kThreads) {
-        const int m = i / COLS, r = i - m * COLS, n = tile * COLS + r;
-        if (n >= p.N) continue;
-        float v = total(m, r);
-        if constexpr (ROWMAJOR) v *= __ldg(sw + n);
-        if constexpr (GATED) {
-          float up = total(m, r + 16);
-          if constexpr (ROWMAJOR) up *= __ldg(sw + p.N + n);
-          v = v / (1.0f + expf(-v)) * up;
-        }
-        store_as(static_cast<T*>(p.out) + (long long)(m0 + m) * p.N + n, v);
-      }
-    }
-    __syncthreads();
-  };
-
-  clear(f);
-  while (tile < p.tiles) {
-#pragma unroll
-    for (int d = 0; d < DEPTH; ++d) {
-      if (tile < p.tiles) {
-        const int u = step * kWarps + warp;
-        if (u < units) {
-          if constexpr (ROWMAJOR) {
-            multiply(ring[d], u, f);
-          } else {
-            float c[MT][NT][4];
-            clear(c);
-            multiply(ring[d], u, c);
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) f[mt][nt][i] = fmaf(c[mt][nt][i], scale[d][mt][i >> 1], f[mt][nt][i]);
-          }
-        }
-        fetch(ring[d], scale[d]);
-        if (++step == steps) {
-          finish();
-          clear(f);
-          step = 0;
-          parity ^= 1;
-          tile += gridDim.x;
-        }
-      }
+    return;
+  }
+  if (with_work > 1) {
+    for (int i = threadIdx.x; i < ntiles * M * 16; i += kThreads) {
+      const int q = i / 16, tile = q / M, at = (tile * k_warps * M + q - tile * M) * 16 + i % 16;
+      part[at] = added(at);
     }
   }
+  ptx::cluster_sync();
+  // every rank adds an equal share of the values
+  const int share = (values + p.ranks - 1) / p.ranks;
+  const uint32_t base = ptx::smem_u32(part);
+  for (int i = rank * share + threadIdx.x; i < min(values, (rank + 1) * share); i += kThreads) {
+    const int r = i % COLS, q = i / COLS, tile = q / M, m = q - tile * M, at = (tile * k_warps * M + m) * 16 + r;
+    float v = 0.f, up = 0.f;
+    for (int k = 0; k < p.ranks; ++k) {
+      const uint32_t from = ptx::mapa_shared(base, k) + 4u * at;
+      float a;
+      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(a) : "r"(from));
+      v += a;
+      if constexpr (GATED) {
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(a) : "r"(from + 32u));
+        up += a;
+      }
+    }
+    finish(tile, m, r, v, up);
+  }
+  ptx::cluster_sync();   // the others may still be reading
 }
 
-template <typename T, int NT, int MT, bool GATED, bool ROWMAJOR>
+template <typename T, int NT, bool GATED, bool ROWMAJOR, bool SMALL>
 int launch_one(const W4A16Params& p, dim3 grid, size_t smem, cudaStream_t st) {
-  constexpr int DEPTH = MT == 2 ? 3 : 4;
-  auto kernel = w4a16_kernel<T, NT, MT, GATED, ROWMAJOR, DEPTH>;
+  auto kernel = w4a16_kernel<T, NT, GATED, ROWMAJOR, SMALL>;
   // the limit belongs to the function, not to a launch: set once, to the most that any call asks for
   static bool configured[64] = {false};
   int dev = 0;
@@ -300,12 +433,44 @@ int launch_one(const W4A16Params& p, dim3 grid, size_t smem, cudaStream_t st) {
   return I4TC_OK;
 }
 
+// Clusters of 1, 2, 4 and 8 blocks that run side by side, a block an SM (148, 74, 33 and 15 here: clusters do not cross a GPC).
+int clusters_at_once(int device, const DeviceInfo* info, int (&out)[4]) {
+  static std::atomic<int> known[64][4];
+  for (int i = 0; i < 4; ++i) {
+    out[i] = known[device][i].load();
+    if (out[i] > 0) continue;
+    if (i == 0) {
+      out[i] = info->sm_count;
+    } else {
+      auto kernel = w4a16_kernel<__nv_bfloat16, 4, false, false, false>;
+      I4TC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kMostSmem));
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(1u, 1u << i, 1);
+      cfg.blockDim = dim3(kThreads, 1, 1);
+      cfg.dynamicSmemBytes = kMostSmem;
+      cudaLaunchAttribute attr;
+      attr.id = cudaLaunchAttributeClusterDimension;
+      attr.val.clusterDim.x = 1;
+      attr.val.clusterDim.y = 1u << i;
+      attr.val.clusterDim.z = 1;
+      cfg.attrs = &attr;
+      cfg.numAttrs = 1;
+      I4TC_CUDA(cudaOccupancyMaxActiveClusters(&out[i], kernel, &cfg));
+      if (out[i] < 1) out[i] = -1;   // this device holds none of that size
+    }
+    known[device][i].store(out[i]);
+  }
+  return I4TC_OK;
+}
+
 template <typename T, bool GATED, bool ROWMAJOR>
 int launch_tokens(const W4A16Params& p, dim3 grid, size_t smem, cudaStream_t st) {
-  const int m = p.M < p.most_tokens ? p.M : p.most_tokens;
-  if (m <= 8) return launch_one<T, 1, 2, GATED, ROWMAJOR>(p, grid, smem, st);
-  if (m <= 16) return launch_one<T, 2, 2, GATED, ROWMAJOR>(p, grid, smem, st);
-  return launch_one<T, 4, 2, GATED, ROWMAJOR>(p, grid, smem, st);
+  if (p.N < (GATED ? 8 : 16)) return launch_one<T, 4, GATED, ROWMAJOR, true>(p, grid, smem, st);
+  switch (token_tiles(p.M < p.most_tokens ? p.M : p.most_tokens, false)) {
+    case 1: return launch_one<T, 1, GATED, ROWMAJOR, false>(p, grid, smem, st);
+    case 2: return launch_one<T, 2, GATED, ROWMAJOR, false>(p, grid, smem, st);
+    default: return launch_one<T, 4, GATED, ROWMAJOR, false>(p, grid, smem, st);
+  }
 }
 
 }  // namespace
@@ -338,20 +503,53 @@ extern "C" int i4tc_w4a16_linear(const void* x, int dtype, int64_t M, int64_t K,
   p.M = (int)M; p.N = (int)N; p.K = (int)K;
   p.rows = gated ? 2 * p.N : p.N;
   p.units = (p.K + 127) / 128;
-  p.tiles = (p.N + (gated ? 15 : 31)) / (gated ? 16 : 32);
+  const int cols = gated ? 8 : 16;
+  const bool small = p.N < cols;
+  p.tiles = (p.N + cols - 1) / cols;
   // as many tokens at a time, up to 32, as a cluster of eight blocks has room for
   p.most_tokens = kMostTokens;
-  while (p.most_tokens > 1 && w4a16_smem(p.most_tokens < p.M ? p.most_tokens : p.M, (p.units + 7) / 8, 2, 8) > kMostSmem) p.most_tokens /= 2;
-  const int tokens = p.M < p.most_tokens ? p.M : p.most_tokens;
-  // K in one block where two blocks' tokens fit an SM, else over the smallest cluster where they do
-  p.ranks = 1;
-  while (p.ranks < 8 && p.ranks * 2 <= p.units && w4a16_smem(tokens, (p.units + p.ranks - 1) / p.ranks, 2, p.ranks) > kMostSmem / 2) p.ranks *= 2;
-  p.units_each = (p.units + p.ranks - 1) / p.ranks;
-  while (p.ranks > 1 && (p.ranks - 1) * p.units_each >= p.units) p.ranks /= 2, p.units_each = (p.units + p.ranks - 1) / p.ranks;
-  const size_t smem = w4a16_smem(tokens, p.units_each, 2, p.ranks);
-  I4TC_REQUIRE(smem <= kMostSmem, I4TC_EUNSUPPORTED, "K is too large");
-  const int slots = info->sm_count * (smem > kMostSmem / 2 ? 1 : 2) / p.ranks;
-  const dim3 grid((unsigned)(p.tiles < slots ? p.tiles : slots), (unsigned)p.ranks, (unsigned)((p.M + p.most_tokens - 1) / p.most_tokens));
+  while (p.most_tokens > 1 && w4a16_smem(p.most_tokens < p.M ? p.most_tokens : p.M, small, (p.units + 7) / 8, 2, 1) > kMostSmem) p.most_tokens /= 2;
+  const int tokens = p.M < p.most_tokens ? p.M : p.most_tokens, chunks = (p.M + p.most_tokens - 1) / p.most_tokens;
+  const int nt = token_tiles(tokens, small);
+  double best = 0;
+  int grid_x = 0;
+  int at_once[4];
+  if (int rc = clusters_at_once(device, info, at_once)) return rc;
+  for (int i = 0; i < 4; ++i) {
+    const int ranks = 1 << i;
+    if (ranks > p.units || at_once[i] < 1) continue;
+    const int each = (p.units + ranks - 1) / ranks;
+    if ((ranks - 1) * each >= p.units) continue;
+    for (int tw = 1; tw <= kWarps; tw *= 2) {
+      const int k_warps = kWarps / tw, steps = (each + k_warps - 1) / k_warps;
+      int gx = at_once[i] > p.tiles ? p.tiles : at_once[i];
+      // partial sums of all of a block's tiles have to fit: else more blocks, in waves
+      int block_tiles = (p.tiles + gx - 1) / gx;
+      while (block_tiles > 1 && w4a16_smem(tokens, small, each, block_tiles, k_warps) > kMostSmem) {
+        gx *= 2;
+        gx = gx > p.tiles ? p.tiles : gx;
+        block_tiles = (p.tiles + gx - 1) / gx;
+      }
+      if (w4a16_smem(tokens, small, each, block_tiles, k_warps) > kMostSmem) continue;
+      const int64_t waves = ((int64_t)gx * chunks + at_once[i] - 1) / at_once[i];
+      const int warp_steps = (block_tiles + tw - 1) / tw * steps;
+      // Microseconds: a step of a block costs its instructions, or a warp's steps their latency; the tokens' rows are laid out by
+      // every block; sums are added per warp that splits K, and between the ranks of a cluster.
+      const double issue = (0.8 * block_tiles * each + 0.2 * kWarps * warp_steps) * (nt == 1 ? 0.033 : nt == 2 ? 0.05 : 0.098);
+      const double latency = warp_steps * 0.35;
+      const double layout = each * tokens * (nt == 1 ? 0.011 : 0.006);
+      const double sums = (double)block_tiles * tokens * 16 * (k_warps - 1) * 0.0005;
+      const double cost = waves * ((issue > latency ? issue : latency) + layout + sums) + (ranks > 1 ? 0.7 : 0.0);
+      if (grid_x == 0 || cost < best) {
+        best = cost;
+        grid_x = gx;
+        p.ranks = ranks; p.units_each = each; p.tile_warps = tw; p.steps = steps;
+      }
+    }
+  }
+  I4TC_REQUIRE(grid_x > 0, I4TC_EUNSUPPORTED, "K is too large");
+  const size_t smem = w4a16_smem(tokens, small, p.units_each, (p.tiles + grid_x - 1) / grid_x, kWarps / p.tile_warps);
+  const dim3 grid((unsigned)grid_x, (unsigned)p.ranks, (unsigned)chunks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   auto pick = [&](auto type) {
     using T = decltype(type);

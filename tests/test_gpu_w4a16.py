@@ -87,6 +87,60 @@ def test_linear_equals_its_tokens_one_by_one():
     assert whole[3].isnan().all() and not whole[20].isfinite().any()
 
 
+@pytest.mark.parametrize("gated", [False, True])
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("per_channel", [False, True])
+def test_numbers_of_very_different_size(per_channel, dtype, gated):
+    """A token's largest number, met by codes of zero, hides nothing of numbers 2^-30 to 2^-100 times as large beside it."""
+    from fp8_inference_toolkit_b200 import ops
+
+    gen = torch.Generator(device="cuda").manual_seed(11)
+    M, K, rows = 5, 1024, 64
+    codes_zero = torch.zeros(K, dtype=torch.bool, device="cuda")
+    codes_zero[5::128] = True
+    x = torch.randn(M, K, device="cuda", generator=gen)
+    x[1] *= 2.0 ** -40 if dtype == torch.bfloat16 else 2.0 ** -13
+    x[2] *= 2.0 ** -100 if dtype == torch.bfloat16 else 2.0 ** -16
+    x[3] *= 2.0 ** 90 if dtype == torch.bfloat16 else 1.0
+    x[:, 5::128] = 60000.0
+    x[4] = 0.0
+    x = x.to(dtype)
+    codes = torch.randint(-8, 8, (rows, K), device="cuda", generator=gen)
+    codes[:, codes_zero] = 0
+    packed = ((codes[:, 0::2] & 15) | ((codes[:, 1::2] & 15) << 4)).to(torch.uint8).contiguous()
+    scale = torch.full((rows,), 2.0 ** -6, device="cuda")
+    if not per_channel:
+        packed, scale = packed.view(rows, K // 128, 64).transpose(0, 1).contiguous(), scale.expand(K // 128, rows).contiguous()
+    ref, slack = _product(x.double() * ~codes_zero, codes.double() * 2.0 ** -6)
+    if not gated:
+        _check(ops.w4a16_linear(x, packed, scale, rows, per_channel), ref, slack)
+        return
+    small = (ref[[0, 1, 2, 4]], slack[[0, 1, 2, 4]])
+    (g, u), (dg, du) = small[0].chunk(2, -1), small[1].chunk(2, -1)
+    out = ops.w4a16_gated_linear(x, packed, scale, rows // 2, per_channel)[[0, 1, 2, 4]]
+    act = g * torch.sigmoid(g)
+    _check(out, act * u, 1.1 * dg * u.abs() + act.abs() * du + (16 + g.abs()) * 2.0 ** -23 * (act * u).abs() + 2.0 ** -126)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_infinities(dtype):
+    """One infinity in a token: its sign times the code's, not a number where the code is zero; other tokens keep their bits."""
+    from fp8_inference_toolkit_b200 import ops
+
+    gen = torch.Generator(device="cuda").manual_seed(12)
+    x = torch.randn(3, 512, device="cuda", generator=gen).to(dtype)
+    packed, scale, w = _weights(gen, 96, 512, False)
+    clean = ops.w4a16_linear(x, packed, scale, 96)
+    x[1, 300] = -float("inf")
+    out = ops.w4a16_linear(x, packed, scale, 96)
+    c = w[:, 300]
+    assert (c == 0).any() and out[1, c == 0].isnan().all()
+    assert torch.equal(out[1, c != 0].double(), -float("inf") * c[c != 0].sign())
+    ref, slack = _product(x[[0, 2]], w)
+    _check(out[[0, 2]], ref, slack)
+    _check(clean[[0, 2]], ref, slack)
+
+
 @pytest.mark.parametrize("layout", ["strided rows", "odd stride", "misaligned", "columns"])
 def test_linear_takes_any_layout_of_tokens(layout):
     from fp8_inference_toolkit_b200 import ops
