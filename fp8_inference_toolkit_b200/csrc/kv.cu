@@ -4,6 +4,7 @@
 // j lies in page block_table[b, j / page_size], row j % page_size.
 #include "common.cuh"
 #include "ptx.cuh"
+#include <math.h>
 #include <math_constants.h>
 #include <type_traits>
 
@@ -104,60 +105,77 @@ struct AttendParams {
   int pages, page_size, table_width;
   int rows, row_tiles;          // of an item: tokens * group
   int parts;                    // blocks
-  float scale_log2;             // scale * log2(e)
+  float scale_log2;             // |scale| * log2(e), not zero: what is masked stays so
+  uint32_t flip;                // sign bits of two queries, where the scale is negative
   unsigned int* status;
 };
 
 __device__ __forceinline__ int cached(const AttendParams& p, int b, bool report) {
   const int n = p.lengths[b];
-  const long long most = min((long long)p.table_width * p.page_size, (long long)INT_MAX - 2 * kTile);
+  const int most = p.table_width * p.page_size;
   if (n >= 0 && n <= most) return n;
   if (report) atomicOr(p.status, kStatusRange);
-  return n < 0 ? 0 : (int)most;
+  return n < 0 ? 0 : most;
 }
 __device__ __forceinline__ int tiles_of(const AttendParams& p, int length) { return (length + p.tokens + kTile - 1) / kTile; }
 
-// Tiles of one (kv head, row tile) over sequences before `upto`, summed by a whole warp.
-__device__ __forceinline__ long long tiles_before(const AttendParams& p, int upto, bool report) {
-  long long n = 0;
-  for (int b = threadIdx.x & 31; b < upto; b += 32) n += tiles_of(p, cached(p, b, report));
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) n += __shfl_xor_sync(0xffffffffu, n, o);
-  return n;
-}
-// The sequence that holds tile `at` of the line (tiles of a sequence: its tiles times `items`), and the line's tiles before it.
-__device__ __forceinline__ int find_sequence(const AttendParams& p, long long at, int items, long long& before) {
-  const int lane = threadIdx.x & 31;
-  long long base = 0;
-  for (int b0 = 0; b0 < p.batch; b0 += 32) {
-    const long long mine = b0 + lane < p.batch ? (long long)tiles_of(p, cached(p, b0 + lane, false)) * items : 0;
-    long long incl = mine;
+// The line, as a whole warp sees it: its length, and where sequences stand in it (a sequence's tiles come `items` times).  With up to 32
+// sequences a lane keeps its own, so that lengths are read once.
+struct Line {
+  int mine, incl, total;   // of the first 32 sequences: this lane's tiles, and those up to it
+  __device__ __forceinline__ void open(const AttendParams& p, int items, bool report) {
+    const int lane = threadIdx.x & 31;
+    mine = lane < p.batch ? tiles_of(p, cached(p, lane, report)) * items : 0;
+    incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-      const long long up = __shfl_up_sync(0xffffffffu, incl, o);
+      const int up = __shfl_up_sync(0xffffffffu, incl, o);
       if (lane >= o) incl += up;
     }
-    const unsigned past = __ballot_sync(0xffffffffu, base + incl > at);
-    if (past) {
-      const int l = __ffs(past) - 1;
-      before = base + __shfl_sync(0xffffffffu, incl - mine, l);
-      return b0 + l;
+    total = __shfl_sync(0xffffffffu, incl, 31);
+    if (p.batch > 32) {
+      int more = 0;
+      for (int b = 32 + lane; b < p.batch; b += 32) more += tiles_of(p, cached(p, b, report)) * items;
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
+      total += more;
     }
-    base += __shfl_sync(0xffffffffu, incl, 31);
   }
-  before = base;
-  return p.batch;
-}
-__device__ __forceinline__ long long part_start(long long total, int parts, int part) { return total / parts * part + total % parts * part / parts; }
-// The part that holds tile `at`: the last whose start is not behind it.
-__device__ __forceinline__ int part_of(long long total, int parts, long long at) {
-  int lo = 0, hi = parts - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) / 2;
-    if (part_start(total, parts, mid) <= at) lo = mid; else hi = mid - 1;
+  // Tiles before sequence `upto`.
+  __device__ __forceinline__ int before(const AttendParams& p, int items, int upto) const {
+    if (upto < 32) return __shfl_sync(0xffffffffu, incl - mine, upto);
+    int more = 0;
+    for (int b = 32 + (threadIdx.x & 31); b < upto; b += 32) more += tiles_of(p, cached(p, b, false)) * items;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
+    return more + __shfl_sync(0xffffffffu, incl, 31);
   }
-  return lo;
-}
+  // The sequence that holds tile `at`, and the tiles before it.
+  __device__ __forceinline__ int find(const AttendParams& p, int items, int at, int& start) const {
+    int b0 = 0, base = 0, m = mine, upto = incl;
+    for (;;) {
+      const unsigned past = __ballot_sync(0xffffffffu, base + upto > at);
+      if (past || b0 + 32 >= p.batch) {
+        const int l = past ? __ffs(past) - 1 : 31;
+        start = base + __shfl_sync(0xffffffffu, upto - m, l);
+        return b0 + l;
+      }
+      base += __shfl_sync(0xffffffffu, upto, 31);
+      b0 += 32;
+      const int lane = threadIdx.x & 31;
+      m = b0 + lane < p.batch ? tiles_of(p, cached(p, b0 + lane, false)) * items : 0;
+      upto = m;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int up = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += up;
+      }
+    }
+  }
+};
+// Part i of the line begins at floor(i total / parts); the part that holds tile `at` is the last whose start is not behind it.
+__device__ __forceinline__ int part_start(int total, int parts, int part) { return total / parts * part + total % parts * part / parts; }
+__device__ __forceinline__ int part_of(int total, int parts, int at) { return (int)(((unsigned long long)(at + 1u) * parts - 1u) / (unsigned)total); }
 
 // Walks the line tile by tile.
 struct Cursor {
@@ -193,32 +211,17 @@ __device__ __forceinline__ void ldmatrix4(uint32_t (&r)[4], uint32_t addr) {
   else
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr) : "memory");
 }
-__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, bool valid) {   // zeros where not valid: nothing is read then
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16u : 0u) : "memory");
+__device__ __forceinline__ void cp_async_16(uint32_t dst, const void* src, uint32_t bytes) {   // 16 bytes, or with 0 zeros: nothing is read then
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-// Two weights in the type of the values, and what they stand for: the sum runs over the rounded weights, so that weights and sum agree.
-template <typename T>
-__device__ __forceinline__ uint32_t pack_weights(float a, float b, float& sum) {
-  if constexpr (std::is_same_v<T, __nv_bfloat16>) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-    const uint32_t u = *reinterpret_cast<const uint32_t*>(&h);
-    sum += __uint_as_float(u << 16) + __uint_as_float(u & 0xFFFF0000u);
-    return u;
-  } else {
-    const __half2 h = __floats2half2_rn(a, b);
-    const float2 f = __half22float2(h);
-    sum += f.x + f.y;
-    return *reinterpret_cast<const uint32_t*>(&h);
-  }
-}
 __device__ __forceinline__ float exp2_fast(float x) {   // 2 ulp, far below the rounding of a weight
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 template <typename T>
-__device__ __forceinline__ uint32_t pack_out(float a, float b) {
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
   if constexpr (std::is_same_v<T, __nv_bfloat16>) {
     const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
     return *reinterpret_cast<const uint32_t*>(&h);
@@ -259,10 +262,12 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
   constexpr int CH = DP / 8;                        // 16-byte chunks of a row
   constexpr int KS = DP / 16, NT = S::KEYS / 8, DT = DP / 8;
   // weights are 2^kLift times exp(score - maximum): a fp16 weight keeps 24 + 12 bits below the largest instead of 24
+  constexpr uint32_t kOnes = std::is_same_v<T, __half> ? 0x3C003C00u : 0x3F803F80u;
   constexpr float kLift = std::is_same_v<T, __half> ? 12.f : 0.f;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t stage0 = ptx::smem_u32(smem);
-  const char** places = reinterpret_cast<const char**>(smem + kStages * 2 * S::kStage);   // [kPlaces][kTile] keys, values
+  ulonglong2* places = reinterpret_cast<ulonglong2*>(smem + kStages * 2 * S::kStage);     // [kPlaces][kTile] keys, values
+  const uint32_t places_at = stage0 + kStages * 2 * S::kStage;
   float* merge = reinterpret_cast<float*>(smem + kStages * 2 * S::kStage + kPlaces * kTile * 16);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wr = warp % WR, wk = warp / WR;
@@ -271,79 +276,85 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
   pdl_trigger();
 
   const int items = p.kv_heads * p.row_tiles;
-  const long long total = tiles_before(p, p.batch, blockIdx.x == 0) * items;
-  const int parts = (int)min((long long)p.parts, total), part = blockIdx.x;   // no part is empty
+  Line line;
+  line.open(p, items, blockIdx.x == 0);
+  const int parts = min(p.parts, line.total), part = blockIdx.x;   // no part is empty
   if (part >= parts) return;
-  const long long first = part_start(total, parts, part);
-  const int count = (int)(part_start(total, parts, part + 1) - first);
+  const int first = part_start(line.total, parts, part), count = part_start(line.total, parts, part + 1) - first;
   Cursor cur;
-  long long before;
-  cur.b = find_sequence(p, first, items, before);
+  int before;
+  cur.b = line.find(p, items, first, before);
   cur.open(p);
-  cur.item = (int)((first - before) / cur.tiles);
-  cur.tile = (int)((first - before) % cur.tiles);
+  cur.item = (first - before) / cur.tiles;
+  cur.tile = (first - before) % cur.tiles;
   Cursor ahead = cur;                               // whose places are looked up next
 
-  // places of the tile at `ahead`: key tid of it
-  auto look_up = [&](const char*& pk, const char*& pv) {
-    pk = pv = nullptr;
+  // Places of the tile at `ahead`: key tid of it.  Where there is none (behind the new tokens, pages out of range) some row that exists.
+  auto look_up = [&]() -> ulonglong2 {
     const int j = ahead.tile * kTile + tid, head = ahead.item / p.row_tiles;
+    const char *k = static_cast<const char*>(p.k), *v = static_cast<const char*>(p.v);
+    long long at = ahead.b * p.new_batch + min(max(j - ahead.length, 0), p.tokens - 1) * p.new_token + head * p.new_head;
     if (j < ahead.length) {
       const int page = p.table[ahead.b * p.table_stride + j / p.page_size];
       if (page >= 0 && page < p.pages) {
-        const long long at = page * p.page_stride + (j % p.page_size) * p.slot_stride + head * p.head_stride;
-        pk = static_cast<const char*>(p.k_cache) + at * 2;
-        pv = static_cast<const char*>(p.v_cache) + at * 2;
+        at = page * p.page_stride + (j % p.page_size) * p.slot_stride + head * p.head_stride;
+        k = static_cast<const char*>(p.k_cache);
+        v = static_cast<const char*>(p.v_cache);
       } else {
         atomicOr(p.status, kStatusRange);
       }
-    } else if (j - ahead.length < p.tokens) {
-      const long long at = ahead.b * p.new_batch + (j - ahead.length) * p.new_token + head * p.new_head;
-      pk = static_cast<const char*>(p.k) + at * 2;
-      pv = static_cast<const char*>(p.v) + at * 2;
     }
+    return make_ulonglong2(reinterpret_cast<unsigned long long>(k + at * 2), reinterpret_cast<unsigned long long>(v + at * 2));
   };
-  auto issue = [&](int i) {                         // tile i of the part into its stage
-    const char** place = places + (i % kPlaces) * kTile * 2;
-    const uint32_t dk = stage0 + (i % kStages) * 2 * S::kStage, dv = dk + S::kStage;
-    const int c = tid % CH;
+  // Tile i of the part into its stage; the first `rows` of its keys exist, the others become zeros.
+  const int my_chunk = tid % CH, my_row = tid / CH;
+  const uint32_t in_head = my_chunk * 8 < p.D ? 16u : 0u;
+  auto issue = [&](int i, int rows) {
+    const uint32_t place = places_at + ((i % kPlaces) * kTile + my_row) * 16;
+    const uint32_t dk = stage0 + (i % kStages) * 2 * S::kStage + my_row * (DP * 2) + ((my_chunk ^ (my_row & 7)) * 16);
+    constexpr int STEP = kAttendThreads / CH;       // rows apart; a multiple of eight, so that the swizzle stays
+    static_assert(STEP % 8 == 0, "rows of a thread share their swizzle");
 #pragma unroll
-    for (int r = tid / CH; r < kTile; r += kAttendThreads / CH) {
-      const char *pk = place[2 * r], *pv = place[2 * r + 1];
-      const bool valid = pk != nullptr && c * 8 < p.D;
-      const uint32_t at = r * (DP * 2) + ((c ^ (r & 7)) * 16);
-      cp_async_16(dk + at, valid ? pk + c * 16 : p.k, valid);
-      cp_async_16(dv + at, valid ? pv + c * 16 : p.v, valid);
+    for (int r = 0; r < kTile; r += STEP) {
+      const uint4 at = ptx::lds128(place + r * 16);
+      const char* pk = reinterpret_cast<const char*>(at.x | (unsigned long long)at.y << 32) + my_chunk * 16;
+      const char* pv = reinterpret_cast<const char*>(at.z | (unsigned long long)at.w << 32) + my_chunk * 16;
+      const uint32_t n = r + my_row < rows ? in_head : 0u;
+      cp_async_16(dk + r * (DP * 2), pk, n);
+      cp_async_16(dk + S::kStage + r * (DP * 2), pv, n);
     }
   };
-  for (int i = 0; i < kStages && i < count; ++i) {
-    if (tid < kTile) {
-      const char *pk, *pv;
-      look_up(pk, pv);
-      places[(i * kTile + tid) * 2] = pk;
-      places[(i * kTile + tid) * 2 + 1] = pv;
+  int rows[kStages];                                // of the tiles ahead: keys that exist
+#pragma unroll
+  for (int i = 0; i < kStages; ++i) {
+    rows[i] = ahead.length + p.tokens - ahead.tile * kTile;
+    if (i < count) {
+      if (tid < kTile) places[i * kTile + tid] = look_up();
+      ahead.next(p);
     }
-    ahead.next(p);
   }
   __syncthreads();
+#pragma unroll
   for (int i = 0; i < kStages - 1; ++i) {
-    if (i < count) issue(i);
+    if (i < count) issue(i, rows[i]);
     asm volatile("cp.async.commit_group;" ::: "memory");
   }
+  int next_rows = rows[kStages - 1];                // of the tile to be issued next
 
   uint32_t q[KS][4];
-  float o[DT][4], m[2], l[2];
+  float o[DT][4], m[2], l[4];                       // m: largest score, not yet scaled; l: sums of the weights (rows g, and 8 + g from l[2])
   int tok[2];                                       // of this lane's two rows; -1 behind the last
   bool begun = true, whole = cur.tile == 0;         // begun: the item's rows have to be set up; whole: this part has it from its start
 
   for (int i = 0; i < count; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     __syncthreads();
-    if (i + kStages - 1 < count) issue(i + kStages - 1);
+    if (i + kStages - 1 < count) issue(i + kStages - 1, next_rows);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    const char *pk = nullptr, *pv = nullptr;
+    ulonglong2 place = make_ulonglong2(0, 0);
     const bool more = i + kStages < count;
-    if (more && tid < kTile) look_up(pk, pv);
+    if (more && tid < kTile) place = look_up();
+    next_rows = ahead.length + p.tokens - ahead.tile * kTile;
 
     if (begun) {
       const int row0 = (cur.item % p.row_tiles) * S::ROWS + wr * 16 + g, kvh = cur.item / p.row_tiles;
@@ -358,10 +369,10 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             const int d = ks * 16 + e * 8 + 2 * t4;
-            q[ks][2 * e + h] = tok[h] >= 0 && d < p.D ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
+            q[ks][2 * e + h] = tok[h] >= 0 && d < p.D ? *reinterpret_cast<const uint32_t*>(src + d) ^ p.flip : 0u;
           }
         m[h] = -CUDART_INF_F;
-        l[h] = 0.f;
+        l[2 * h] = l[2 * h + 1] = 0.f;
       }
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt)
@@ -387,10 +398,6 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
         mma<T>(s[2 * np], q[ks], b[0], b[1]);
         mma<T>(s[2 * np + 1], q[ks], b[2], b[3]);
       }
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) s[nt][k] *= p.scale_log2;
     const int j0 = cur.tile * kTile;
     const bool edge = j0 + kTile > cur.length;      // the tile holds new tokens, or what is behind them
     bool odd = false;
@@ -441,14 +448,19 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
     for (int h = 0; h < 2; ++h) {
       top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
       top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-      base[h] = top[h] == -CUDART_INF_F ? 0.f : top[h] - kLift;
-      const float fade = exp2_fast(m[h] - (base[h] + kLift));
-      m[h] = top[h];
-      l[h] *= fade;
+      base[h] = top[h] == -CUDART_INF_F ? 0.f : top[h] * p.scale_log2 - kLift;
+    }
+    if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
 #pragma unroll
-      for (int dt = 0; dt < DT; ++dt) {
-        o[dt][2 * h] *= fade;
-        o[dt][2 * h + 1] *= fade;
+      for (int h = 0; h < 2; ++h) {
+        const float fade = m[h] == top[h] ? 1.f : exp2_fast((m[h] - top[h]) * p.scale_log2);
+        m[h] = top[h];
+        l[2 * h] *= fade;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          o[dt][2 * h] *= fade;
+          o[dt][2 * h + 1] *= fade;
+        }
       }
     }
     if (odd) {                                      // what was taken out of the values goes to the rows that see it
@@ -478,10 +490,11 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        w[nt][h] = pack_weights<T>(exp2_fast(s[nt][2 * h] - base[h]), exp2_fast(s[nt][2 * h + 1] - base[h]), l[h]);
+        w[nt][h] = pack_pair<T>(exp2_fast(fmaf(s[nt][2 * h], p.scale_log2, -base[h])), exp2_fast(fmaf(s[nt][2 * h + 1], p.scale_log2, -base[h])));
 #pragma unroll
     for (int kk = 0; kk < NT / 2; ++kk) {
       const uint32_t a[4] = {w[2 * kk][0], w[2 * kk][1], w[2 * kk + 1][0], w[2 * kk + 1][1]};
+      mma<T>(l, a, kOnes, kOnes);                   // the sums of the weights as they were rounded
 #pragma unroll
       for (int dp = 0; dp < DT / 2; ++dp) {
         uint32_t b[4];
@@ -494,11 +507,8 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
 
     const bool ends = cur.tile + 1 == cur.tiles;
     if (ends || i + 1 == count) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      }
+      m[0] *= p.scale_log2;
+      m[1] *= p.scale_log2;
       if constexpr (S::WK > 1) {
         // the key warps, one after the other and half of the elements at a time, into the first
         float* mo = merge + (wr * 16 + g) * (DP / 2) + 2 * t4;
@@ -515,7 +525,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
                 for (int dt = 0; dt < DT / 2; ++dt)
                   *reinterpret_cast<float2*>(mo + 8 * h * (DP / 2) + dt * 8) =
                       make_float2(o[half * (DT / 2) + dt][2 * h], o[half * (DT / 2) + dt][2 * h + 1]);
-                if (half == 0 && t4 == 0) *reinterpret_cast<float2*>(ml + 16 * h) = make_float2(m[h], l[h]);
+                if (half == 0 && t4 == 0) *reinterpret_cast<float2*>(ml + 16 * h) = make_float2(m[h], l[2 * h]);
               }
             }
             __syncthreads();
@@ -528,7 +538,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
                   fa[h] = exp2_fast(m[h] - zero);
                   fb[h] = exp2_fast(his.x - zero);
                   m[h] = both;
-                  l[h] = l[h] * fa[h] + his.y * fb[h];
+                  l[2 * h] = l[2 * h] * fa[h] + his.y * fb[h];
                 }
 #pragma unroll
                 for (int dt = 0; dt < DT / 2; ++dt) {
@@ -549,12 +559,12 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
           for (int h = 0; h < 2; ++h) {
             const int row = row0 + 8 * h;
             if (tok[h] < 0) continue;
-            const float inv = inverse_sum(p, l[h], cur.b, tok[h], cur.length);
+            const float inv = inverse_sum(p, l[2 * h], cur.b, tok[h], cur.length);
             T* dst = static_cast<T*>(p.out) + (((long long)cur.b * p.tokens + tok[h]) * p.heads + kvh * p.group + row % p.group) * p.D;
 #pragma unroll
             for (int dt = 0; dt < DT; ++dt) {
               const int d = dt * 8 + 2 * t4;
-              if (d < p.D) *reinterpret_cast<uint32_t*>(dst + d) = pack_out<T>(o[dt][2 * h] * inv, o[dt][2 * h + 1] * inv);
+              if (d < p.D) *reinterpret_cast<uint32_t*>(dst + d) = pack_pair<T>(o[dt][2 * h] * inv, o[dt][2 * h + 1] * inv);
             }
           }
         } else {
@@ -566,7 +576,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
             const int row = wr * 16 + g + 8 * h;
             if (t4 == 0) {
               slot[row] = m[h];
-              slot[S::ROWS + row] = l[h];
+              slot[S::ROWS + row] = l[2 * h];
             }
             float* dst = slot + 2 * S::ROWS + row * DP + 2 * t4;
 #pragma unroll
@@ -578,44 +588,45 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
     }
     cur.next(p);
     if (more) {
-      if (tid < kTile) {
-        const int at = ((i + kStages) % kPlaces) * kTile + tid;
-        places[2 * at] = pk;
-        places[2 * at + 1] = pv;
-      }
+      if (tid < kTile) places[((i + kStages) % kPlaces) * kTile + tid] = place;
       ahead.next(p);
     }
   }
 }
 
-// Items that no part held whole: their parts in ascending order.  A warp takes a row, a lane DP / 32 consecutive elements.
+// Items that no part held whole: their parts in ascending order.  A block takes a row: its warps a quarter of the parts each, which are
+// added in order in the end; a lane DP / 32 consecutive elements.
 template <typename T, int DP>
 __global__ void __launch_bounds__(kAttendThreads) attend_join_kernel(const AttendParams p, int tile_rows) {
-  constexpr int E = DP / 32;
+  constexpr int E = DP / 32, WARPS = kAttendThreads / 32;
+  __shared__ float sums[WARPS][DP + 2];
   pdl_wait();
-  const int lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int items = p.kv_heads * p.row_tiles;
-  const int b = blockIdx.x / items, item = blockIdx.x % items;
-  const int row = blockIdx.y * (kAttendThreads / 32) + (threadIdx.x >> 5);
+  const int b = blockIdx.x / items, item = blockIdx.x % items, row = blockIdx.y;
   const int at_row = (item % p.row_tiles) * tile_rows + row;
+  if (at_row >= p.rows) return;
+  Line line;
+  line.open(p, items, false);
   const int length = cached(p, b, false), tiles = tiles_of(p, length);
-  const long long total = tiles_before(p, p.batch, false) * items, start = tiles_before(p, b, false) * items + (long long)item * tiles;
-  const int parts = (int)min((long long)p.parts, total);
-  const int first = part_of(total, parts, start), last = part_of(total, parts, start + tiles - 1);
-  if (first == last || row >= tile_rows || at_row >= p.rows) return;
+  const int start = line.before(p, items, b) + item * tiles;
+  const int parts = min(p.parts, line.total);
+  const int first = part_of(line.total, parts, start), last = part_of(line.total, parts, start + tiles - 1);
+  if (first == last) return;
   const size_t step = 2 * slot_floats(tile_rows, DP);
-  const float* opening = p.scratch + first * step + (part_start(total, parts, first) == start ? 0 : step / 2);
+  const float* opening = p.scratch + first * step + (part_start(line.total, parts, first) == start ? 0 : step / 2);
   auto slot = [&](int part) { return part == first ? opening : p.scratch + part * step; };
-  float top = -CUDART_INF_F;
-  for (int part = first + lane; part <= last; part += 32) top = fmaxf(top, slot(part)[row]);
+  const int count = last - first + 1, each = (count + WARPS - 1) / WARPS;
+  const int from = first + min(count, warp * each), to = first + min(count, (warp + 1) * each);
+  float top = -CUDART_INF_F, sum = 0.f, v[E];
+  for (int part = from + lane; part < to; part += 32) top = fmaxf(top, slot(part)[row]);
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
   const float zero = top == -CUDART_INF_F ? 0.f : top;
-  float sum = 0.f, v[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) v[e] = 0.f;
-#pragma unroll 4
-  for (int part = first; part <= last; ++part) {
+#pragma unroll 8
+  for (int part = from; part < to; ++part) {
     const float* s = slot(part);
     const float f = exp2_fast(s[row] - zero);
     sum += s[tile_rows + row] * f;
@@ -628,12 +639,32 @@ __global__ void __launch_bounds__(kAttendThreads) attend_join_kernel(const Atten
       v[0] += x.x * f; v[1] += x.y * f;
     }
   }
-  const int t = at_row / p.group, head = (item / p.row_tiles) * p.group + at_row % p.group;
-  const float inv = inverse_sum(p, sum, b, t, length);
-  T* dst = static_cast<T*>(p.out) + (((long long)b * p.tokens + t) * p.heads + head) * p.D + lane * E;
 #pragma unroll
-  for (int e = 0; e < E; e += 2)
-    if (lane * E + e < p.D) *reinterpret_cast<uint32_t*>(dst + e) = pack_out<T>(v[e] * inv, v[e + 1] * inv);
+  for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = v[e];
+  if (lane == 0) {
+    sums[warp][DP] = top;
+    sums[warp][DP + 1] = sum;
+  }
+  __syncthreads();
+  float all = -CUDART_INF_F;
+#pragma unroll
+  for (int k = 0; k < WARPS; ++k) all = fmaxf(all, sums[k][DP]);
+  const float base = all == -CUDART_INF_F ? 0.f : all;
+  const int d = threadIdx.x;
+  float x = 0.f;
+  sum = 0.f;
+#pragma unroll
+  for (int k = 0; k < WARPS; ++k) {
+    const float f = exp2_fast(sums[k][DP] - base);
+    sum += sums[k][DP + 1] * f;
+    if (d < DP) x += sums[k][d] * f;
+  }
+  const int t = at_row / p.group, head = (item / p.row_tiles) * p.group + at_row % p.group;
+  if (d < p.D) {
+    const float y = x * inverse_sum(p, sum, b, t, length);
+    T* dst = static_cast<T*>(p.out) + (((long long)b * p.tokens + t) * p.heads + head) * p.D + d;
+    if constexpr (std::is_same_v<T, __half>) *dst = __float2half_rn(y); else *dst = __float2bfloat16_rn(y);
+  }
 }
 
 int row_warps(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
@@ -655,7 +686,7 @@ int launch_attend(const AttendParams& p, cudaStream_t st) {
     if (dev < 64) configured[dev] = true;
   }
   I4TC_CUDA(launch_kernel(true, kernel, dim3((unsigned)p.parts), kAttendThreads, S::kSmem, st, p));
-  const dim3 grid((unsigned)(p.batch * p.kv_heads * p.row_tiles), (unsigned)((S::ROWS < p.rows ? S::ROWS : p.rows) + 3) / 4);
+  const dim3 grid((unsigned)(p.batch * p.kv_heads * p.row_tiles), (unsigned)(S::ROWS < p.rows ? S::ROWS : p.rows));
   I4TC_CUDA(launch_kernel(true, attend_join_kernel<T, DP>, grid, kAttendThreads, 0, st, p, S::ROWS));
   return I4TC_OK;
 }
@@ -714,11 +745,13 @@ extern "C" int i4tc_tree_attention(const i4tc_tree_attention_args* a, int device
   const int warps = row_warps(rows);
   p.rows = (int)rows; p.row_tiles = (int)((rows + 16 * warps - 1) / (16 * warps));
   const int64_t items = (int64_t)p.kv_heads * p.row_tiles;
-  I4TC_REQUIRE(a->batch * items < (1ll << 31), I4TC_EINVAL, "too many heads");
   const int64_t most_length = a->table_width * a->page_size;
+  I4TC_REQUIRE(most_length < (1ll << 31) - 2 * kTile && a->batch * items * ((most_length + a->tokens) / kTile + 1) < (1ll << 31), I4TC_EUNSUPPORTED,
+               "the table has room for too many tokens");
   p.parts = attend_parts(info->sm_count, a->batch, items, most_length, a->tokens);
   I4TC_REQUIRE(a->scratch_bytes >= (int64_t)p.parts * 2 * (int64_t)slot_floats(16 * warps, padded_dim(p.D)) * 4, I4TC_EWORKSPACE, "the scratch is too small");
-  p.scale_log2 = (float)(a->scale * 1.4426950408889634);
+  p.scale_log2 = fmaxf((float)(fabs(a->scale) * 1.4426950408889634), 1e-30f);
+  p.flip = a->scale < 0 ? 0x80008000u : 0u;
   p.status = info->status;
   DeviceGuard guard(device);
   I4TC_CUDA(guard.err);
