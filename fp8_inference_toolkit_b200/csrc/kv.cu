@@ -261,9 +261,10 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
   using S = AttendShape<DP, WR>;
   constexpr int CH = DP / 8;                        // 16-byte chunks of a row
   constexpr int KS = DP / 16, NT = S::KEYS / 8, DT = DP / 8;
-  // weights are 2^kLift times exp(score - maximum): a fp16 weight keeps 24 + 12 bits below the largest instead of 24
+  // Weights are 2^kLift exp(score - m), where m is the largest score up to the last time that a larger one was more than 2^kSlack times
+  // its weight: results are seldom scaled anew.  A fp16 weight goes up to 2^14 and keeps 24 + 8 bits below m's.
   constexpr uint32_t kOnes = std::is_same_v<T, __half> ? 0x3C003C00u : 0x3F803F80u;
-  constexpr float kLift = std::is_same_v<T, __half> ? 12.f : 0.f;
+  constexpr float kLift = std::is_same_v<T, __half> ? 8.f : 0.f, kSlack = std::is_same_v<T, __half> ? 6.f : 8.f;
   extern __shared__ __align__(128) uint8_t smem[];
   const uint32_t stage0 = ptx::smem_u32(smem);
   ulonglong2* places = reinterpret_cast<ulonglong2*>(smem + kStages * 2 * S::kStage);     // [kPlaces][kTile] keys, values
@@ -289,13 +290,17 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
   cur.tile = (first - before) % cur.tiles;
   Cursor ahead = cur;                               // whose places are looked up next
 
-  // Places of the tile at `ahead`: key tid of it.  Where there is none (behind the new tokens, pages out of range) some row that exists.
-  auto look_up = [&]() -> ulonglong2 {
+  // Places of the tile at `ahead`: key tid of it.  In two halves, the page's number and the addresses, so that nobody waits for the table.
+  // Where there is no place (behind the new tokens, pages out of range) some row that exists.
+  auto look_up = [&]() -> int {
+    const int j = ahead.tile * kTile + tid;
+    return j < ahead.length ? __ldg(p.table + ahead.b * p.table_stride + j / p.page_size) : 0;
+  };
+  auto place_of = [&](int page) -> ulonglong2 {
     const int j = ahead.tile * kTile + tid, head = ahead.item / p.row_tiles;
     const char *k = static_cast<const char*>(p.k), *v = static_cast<const char*>(p.v);
     long long at = ahead.b * p.new_batch + min(max(j - ahead.length, 0), p.tokens - 1) * p.new_token + head * p.new_head;
     if (j < ahead.length) {
-      const int page = p.table[ahead.b * p.table_stride + j / p.page_size];
       if (page >= 0 && page < p.pages) {
         at = page * p.page_stride + (j % p.page_size) * p.slot_stride + head * p.head_stride;
         k = static_cast<const char*>(p.k_cache);
@@ -329,7 +334,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
   for (int i = 0; i < kStages; ++i) {
     rows[i] = ahead.length + p.tokens - ahead.tile * kTile;
     if (i < count) {
-      if (tid < kTile) places[i * kTile + tid] = look_up();
+      if (tid < kTile) places[i * kTile + tid] = place_of(look_up());
       ahead.next(p);
     }
   }
@@ -342,18 +347,29 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
   int next_rows = rows[kStages - 1];                // of the tile to be issued next
 
   uint32_t q[KS][4];
-  float o[DT][4], m[2], l[4];                       // m: largest score, not yet scaled; l: sums of the weights (rows g, and 8 + g from l[2])
+  float o[DT][4], m[2], l[4];                       // m: reference of the weights, not yet scaled; l: sums of the weights (rows g, and 8 + g from l[2])
   int tok[2];                                       // of this lane's two rows; -1 behind the last
+  // Where this lane reads a tile's keys and values for ldmatrix: chunk c of a row stands at c ^ (row & 7), so chunks 2 j + {0, 1} of eight
+  // are four addresses, and the rest (other rows, the next eight chunks) is added to them.
+  const int key0 = wk * S::KEYS;                    // this warp's keys in a tile
+  uint32_t k_at[4], v_at[4];
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const int kr = key0 + (lane & 7) + ((lane >> 4) & 1) * 8, vr = key0 + (lane & 15);
+    k_at[j] = stage0 + kr * (DP * 2) + (((2 * j + ((lane >> 3) & 1)) ^ (kr & 7)) * 16);
+    v_at[j] = stage0 + S::kStage + vr * (DP * 2) + (((2 * j + (lane >> 4)) ^ (vr & 7)) * 16);
+  }
   bool begun = true, whole = cur.tile == 0;         // begun: the item's rows have to be set up; whole: this part has it from its start
 
+  int stage = 0;                                    // of tile i
   for (int i = 0; i < count; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     __syncthreads();
     if (i + kStages - 1 < count) issue(i + kStages - 1, next_rows);
     asm volatile("cp.async.commit_group;" ::: "memory");
-    ulonglong2 place = make_ulonglong2(0, 0);
     const bool more = i + kStages < count;
-    if (more && tid < kTile) place = look_up();
+    int page = 0;
+    if (more && tid < kTile) page = look_up();
     next_rows = ahead.length + p.tokens - ahead.tile * kTile;
 
     if (begun) {
@@ -381,8 +397,8 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
       begun = false;
     }
 
-    const uint32_t sk = stage0 + (i % kStages) * 2 * S::kStage, sv = sk + S::kStage;
-    const int key0 = wk * S::KEYS;                  // of this warp, in the tile
+    const uint32_t at_stage = stage * 2 * S::kStage, sv = stage0 + at_stage + S::kStage;
+    if (++stage == kStages) stage = 0;
     float s[NT][4];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -393,8 +409,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
 #pragma unroll
       for (int np = 0; np < NT / 2; ++np) {
         uint32_t b[4];
-        const int row = key0 + np * 16 + (lane & 7) + ((lane >> 4) & 1) * 8, c = ks * 2 + ((lane >> 3) & 1);
-        ldmatrix4<false>(b, sk + row * (DP * 2) + ((c ^ (row & 7)) * 16));
+        ldmatrix4<false>(b, k_at[ks & 3] + at_stage + (np * 16 * (DP * 2) + (ks >> 2) * 128));
         mma<T>(s[2 * np], q[ks], b[0], b[1]);
         mma<T>(s[2 * np + 1], q[ks], b[2], b[3]);
       }
@@ -444,13 +459,14 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
 #pragma unroll
       for (int k = 0; k < 4; ++k) top[k >> 1] = fmaxf(top[k >> 1], s[nt][k]);
     float base[2];
+    bool rise = false;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 1));
       top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], 2));
-      base[h] = top[h] == -CUDART_INF_F ? 0.f : top[h] * p.scale_log2 - kLift;
+      rise |= m[h] == -CUDART_INF_F ? top[h] != m[h] : (top[h] - m[h]) * p.scale_log2 > kSlack;
     }
-    if (__any_sync(0xffffffffu, top[0] != m[0] || top[1] != m[1])) {
+    if (__any_sync(0xffffffffu, rise)) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         const float fade = m[h] == top[h] ? 1.f : exp2_fast((m[h] - top[h]) * p.scale_log2);
@@ -463,6 +479,8 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
         }
       }
     }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) base[h] = m[h] == -CUDART_INF_F ? 0.f : m[h] * p.scale_log2 - kLift;
     if (odd) {                                      // what was taken out of the values goes to the rows that see it
       for (int key = key0; key < key0 + S::KEYS; ++key) {
         const int j = j0 + key - cur.length;
@@ -498,8 +516,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
 #pragma unroll
       for (int dp = 0; dp < DT / 2; ++dp) {
         uint32_t b[4];
-        const int row = key0 + kk * 16 + (lane & 15), c = dp * 2 + (lane >> 4);
-        ldmatrix4<true>(b, sv + row * (DP * 2) + ((c ^ (row & 7)) * 16));
+        ldmatrix4<true>(b, v_at[dp & 3] + at_stage + (kk * 16 * (DP * 2) + (dp >> 2) * 128));
         mma<T>(o[2 * dp], a, b[0], b[1]);
         mma<T>(o[2 * dp + 1], a, b[2], b[3]);
       }
@@ -588,7 +605,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
     }
     cur.next(p);
     if (more) {
-      if (tid < kTile) places[((i + kStages) % kPlaces) * kTile + tid] = place;
+      if (tid < kTile) places[((i + kStages) % kPlaces) * kTile + tid] = place_of(page);
       ahead.next(p);
     }
   }

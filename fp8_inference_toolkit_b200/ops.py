@@ -529,25 +529,50 @@ def _half_input(t: torch.Tensor, name: str, dim: int) -> None:
     _require(not (t.requires_grad and torch.is_grad_enabled()), f"{name} requires grad: the op has no backward pass, call it under torch.no_grad()")
 
 
-def _w4a16(x: torch.Tensor, w_packed: torch.Tensor, w_scale: torch.Tensor, N: int, per_channel: bool, gated: bool, who: str) -> torch.Tensor:
+_HALF = {torch.bfloat16: _cabi.BF16, torch.float16: _cabi.FP16}
+# The ops below are called once or more a layer for a single token, where a microsecond of checks is a tenth of the call: what a good call
+# looks like is one expression, and the checks that name what is wrong run for the others.
+
+
+def _check_w4a16(x, w_packed, w_scale, rows, per_channel) -> None:
     _half_input(x, "input", 2)
-    M, K = x.shape
+    K = x.shape[1]
     if per_channel:
         _require(K > 0 and K % 64 == 0, "K must be a multiple of 64")
     else:
         _require(K > 0 and K % 128 == 0, "K must be divisible by group_size")
-    rows = 2 * N if gated else N
     _require(w_packed.device == x.device and w_scale.device == x.device, "all tensors must be on the same device")
     _require(w_packed.dtype == torch.uint8 and w_packed.is_contiguous(), "b_packed must be contiguous uint8")
     _require(w_packed.numel() == rows * (K // 2), "b_packed does not have rows*K/2 bytes")
     _require(w_scale.dtype == torch.float32 and w_scale.is_contiguous(), "scale_b must be contiguous float32")
     _require(w_scale.numel() == (rows if per_channel else K // 128 * rows), "scale_b does not have a scale for every row (and group)")
-    ldx = x.stride(0) if M > 1 else K
-    if x.stride(1) != 1 or ldx % 8 or x.data_ptr() % 16:
+    raise RuntimeError("w4a16_linear: unsupported arguments")
+
+
+def _w4a16(x: torch.Tensor, w_packed: torch.Tensor, w_scale: torch.Tensor, N: int, per_channel: bool, gated: bool, who: str) -> torch.Tensor:
+    rows = 2 * N if gated else N
+    code = _HALF.get(x.dtype)
+    if code is None or x.dim() != 2:
+        _check_w4a16(x, w_packed, w_scale, rows, per_channel)
+    M, K = x.shape
+    index = x.get_device()
+    if not (index >= 0 and K > 0 and K % (64 if per_channel else 128) == 0 and w_packed.get_device() == index and w_scale.get_device() == index
+            and w_packed.dtype is torch.uint8 and w_scale.dtype is torch.float32 and w_packed.is_contiguous() and w_scale.is_contiguous()
+            and w_packed.numel() * 2 == rows * K and w_scale.numel() == (rows if per_channel else K // 128 * rows)
+            and not (x.requires_grad and torch.is_grad_enabled())):
+        _check_w4a16(x, w_packed, w_scale, rows, per_channel)
+    at = x.data_ptr()
+    ldx, inner = x.stride()
+    if M <= 1:
+        ldx = K
+    if inner != 1 or ldx % 8 or at % 16:
         x, ldx = x.clone(memory_format=torch.contiguous_format), K
-    out = torch.empty((M, N), dtype=x.dtype, device=x.device)
-    check(lib.i4tc_w4a16_linear(x.data_ptr(), _DTYPES[x.dtype], M, K, ldx, w_packed.data_ptr(), w_scale.data_ptr(), per_channel, gated,
-                                out.data_ptr(), N, _dev(x), _stream(x)), who)
+        at = x.data_ptr()
+    out = x.new_empty((M, N))
+    rc = lib.i4tc_w4a16_linear(at, code, M, K, ldx, w_packed.data_ptr(), w_scale.data_ptr(), per_channel, gated, out.data_ptr(), N, index,
+                               _raw_stream(index) if _raw_stream is not None else _stream(x))
+    if rc:
+        check(rc, who)
     return out
 
 
@@ -589,15 +614,27 @@ def rope_frequencies(rotary_dim: int, theta: float, device="cuda", scaling: str 
     return torch.tensor(freqs, dtype=torch.float64, device=device), scale
 
 
-def _rope(x, positions, freqs, interleaved, scale, inverse, in_place, who):
+def _check_rope(x, positions, freqs) -> None:
     _half_input(x, "x", 3)
-    tokens, heads, D = x.shape
+    tokens, _, D = x.shape
     _require(positions.dim() == 1 and positions.numel() == tokens, "positions must be [tokens]")
     _require(positions.dtype == torch.int64 or positions.dtype == torch.int32, "positions must be int32 or int64")
     _require(freqs.dtype == torch.float64 and freqs.dim() == 1 and freqs.is_contiguous(), "freqs must be a contiguous 1D float64 tensor")
-    R = 2 * freqs.numel()
-    _require(R <= D, "a head has fewer elements than the frequencies rotate")
+    _require(2 * freqs.numel() <= D, "a head has fewer elements than the frequencies rotate")
     _require(positions.device == x.device and freqs.device == x.device, "all tensors must be on the same device")
+    raise RuntimeError("rope: unsupported arguments")
+
+
+def _rope(x, positions, freqs, interleaved, scale, inverse, in_place, who):
+    code = _HALF.get(x.dtype)
+    if code is None or x.dim() != 3:
+        _check_rope(x, positions, freqs)
+    tokens, heads, D = x.shape
+    index, kind, R = x.get_device(), positions.dtype, 2 * freqs.numel()
+    if not (index >= 0 and positions.get_device() == index and freqs.get_device() == index and positions.dim() == 1 and positions.numel() == tokens
+            and (kind is torch.int64 or kind is torch.int32) and freqs.dtype is torch.float64 and freqs.dim() == 1 and freqs.is_contiguous()
+            and R <= D and not (x.requires_grad and torch.is_grad_enabled())):
+        _check_rope(x, positions, freqs)
     if not positions.is_contiguous():
         positions = positions.contiguous()
     st, sh, sd = x.stride()
@@ -611,17 +648,19 @@ def _rope(x, positions, freqs, interleaved, scale, inverse, in_place, who):
         if sd != 1 and D > 1:
             x = x.contiguous()
             st, sh, sd = x.stride()
-        out = torch.empty((tokens, heads, D), dtype=x.dtype, device=x.device)
+        out = x.new_empty((tokens, heads, D))
         ot, oh = heads * D, D
-        if out.numel() == 0:
-            return out
+    if out.numel() == 0:
+        return out
     # the stride of an axis of one counts for nothing
     if tokens == 1:
         st = ot = heads * D
     if heads == 1:
         sh = oh = D
-    check(lib.i4tc_rope(x.data_ptr(), _DTYPES[x.dtype], tokens, heads, D, R, st, sh, positions.data_ptr(), positions.dtype == torch.int64,
-                        freqs.data_ptr(), interleaved, scale, inverse, out.data_ptr(), ot, oh, _dev(x), _stream(x)), who)
+    rc = lib.i4tc_rope(x.data_ptr(), code, tokens, heads, D, R, st, sh, positions.data_ptr(), kind is torch.int64, freqs.data_ptr(), interleaved,
+                       scale, inverse, out.data_ptr(), ot, oh, index, _raw_stream(index) if _raw_stream is not None else _stream(x))
+    if rc:
+        check(rc, who)
     return out
 
 
@@ -645,12 +684,9 @@ _ATTENTION_ARGS = struct.Struct("@10P21qd")
 _APPEND_ARGS = struct.Struct("@8P16q")
 
 
-def _cache_pair(k_cache, v_cache, block_table, lengths, k, v):
-    """Checks of a paged cache and the new rows beside it; (k, v) with the same strides."""
-    _half_input(k, "k", 4)
-    _half_input(v, "v", 4)
-    _half_input(k_cache, "k_cache", 4)
-    _half_input(v_cache, "v_cache", 4)
+def _check_cache(k_cache, v_cache, block_table, lengths, k, v) -> None:
+    for t, name in ((k, "k"), (v, "v"), (k_cache, "k_cache"), (v_cache, "v_cache")):
+        _half_input(t, name, 4)
     _require(k.shape == v.shape, "k and v must have the same shape")
     _require(k_cache.shape == v_cache.shape and k_cache.stride() == v_cache.stride(), "k_cache and v_cache must have the same shape and strides")
     _require(k.dtype == v.dtype == k_cache.dtype == v_cache.dtype, "keys, values and cache must have the same dtype")
@@ -663,9 +699,32 @@ def _cache_pair(k_cache, v_cache, block_table, lengths, k, v):
     dev = k.device
     _require(v.device == dev and k_cache.device == dev and v_cache.device == dev and block_table.device == dev and lengths.device == dev,
              "all tensors must be on the same device")
-    if k.stride() != v.stride() or k.stride(3) != 1:
+    raise RuntimeError("unsupported arguments")
+
+
+def _cache_pair(k_cache, v_cache, block_table, lengths, k, v):
+    """Checks of a paged cache and the new rows beside it; (k, v, their strides, cache strides, block_table, lengths), k and v with the same strides."""
+    kind, index = k.dtype, k.get_device()
+    if not (kind in _HALF and index >= 0 and k.dim() == 4 and k_cache.dim() == 4 and block_table.dim() == 2 and lengths.dim() == 1):
+        _check_cache(k_cache, v_cache, block_table, lengths, k, v)
+    B, _, H, D = shape = k.shape
+    _, page, cache_heads, cache_D = cache_shape = k_cache.shape
+    new, cache = k.stride(), k_cache.stride()
+    if not (v.dtype is kind and k_cache.dtype is kind and v_cache.dtype is kind and v.shape == shape and v_cache.shape == cache_shape
+            and v_cache.stride() == cache and H == cache_heads and D == cache_D and page > 0 and (cache[3] == 1 or D <= 1)
+            and block_table.dtype is torch.int32 and lengths.dtype is torch.int32 and block_table.shape[0] == B and lengths.shape[0] == B
+            and v.get_device() == index and k_cache.get_device() == index and v_cache.get_device() == index
+            and block_table.get_device() == index and lengths.get_device() == index
+            and not ((k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad) and torch.is_grad_enabled())):
+        _check_cache(k_cache, v_cache, block_table, lengths, k, v)
+    if v.stride() != new or new[3] != 1:
         k, v = k.contiguous(), v.contiguous()
-    return k, v, block_table if block_table.stride(1) == 1 or block_table.shape[1] <= 1 else block_table.contiguous(), lengths.contiguous()
+        new = k.stride()
+        if v.stride() != new:   # axes of one element: any stride counts as contiguous
+            v = v.as_strided(shape, new)
+    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+        block_table = block_table.contiguous()
+    return k, v, new, cache, block_table, lengths if lengths.is_contiguous() else lengths.contiguous()
 
 
 def kv_cache_append_(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
@@ -675,22 +734,28 @@ def kv_cache_append_(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tens
     ``block_table[b, token // page_size]``, and comes from new row ``select[b, i]`` (``i`` without ``select``): a prompt, or the accepted path
     of a tree of drafts.  All index tensors int32.  ``lengths`` stay as they are.  Counts, rows, tokens and pages out of range
     write nothing and are raised by ``check_status``."""
-    k, v, block_table, lengths = _cache_pair(k_cache, v_cache, block_table, lengths, k, v)
+    k, v, new, cache, block_table, lengths = _cache_pair(k_cache, v_cache, block_table, lengths, k, v)
     B, T, H, D = k.shape
+    index = k.get_device()
+    counts_at = select_at = select_stride = 0
     if counts is not None:
-        _require(counts.dtype == torch.int32 and counts.dim() == 1 and counts.shape[0] == B and counts.device == k.device, "counts must be int32 [batch]")
+        _require(counts.dtype is torch.int32 and counts.dim() == 1 and counts.shape[0] == B and counts.get_device() == index, "counts must be int32 [batch]")
         counts = counts.contiguous()
+        counts_at = counts.data_ptr()
     if select is not None:
-        _require(select.dtype == torch.int32 and select.dim() == 2 and select.shape[0] == B and select.device == k.device, "select must be int32 [batch, new rows]")
+        _require(select.dtype is torch.int32 and select.dim() == 2 and select.shape[0] == B and select.get_device() == index,
+                 "select must be int32 [batch, new rows]")
         _require(select.shape[1] >= T, "select must have as many columns as there are new rows")
         if select.stride(1) != 1:
             select = select.contiguous()
-    new, cache = k.stride(), k_cache.stride()
+        select_at, select_stride = select.data_ptr(), select.stride(0)
+    pages, page = k_cache.shape[:2]
     args = _APPEND_ARGS.pack(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
-                             0 if counts is None else counts.data_ptr(), 0 if select is None else select.data_ptr(),
-                             2, B, T, H, D, k_cache.shape[0], k_cache.shape[1], block_table.shape[1], new[0], new[1], new[2], cache[0], cache[1],
-                             cache[2], block_table.stride(0), 0 if select is None else select.stride(0))
-    check(lib.i4tc_kv_append(args, _dev(k), _stream(k)), "kv_cache_append_")
+                             counts_at, select_at, 2, B, T, H, D, pages, page, block_table.shape[1], new[0], new[1], new[2], cache[0], cache[1],
+                             cache[2], block_table.stride(0), select_stride)
+    rc = lib.i4tc_kv_append(args, index, _raw_stream(index) if _raw_stream is not None else _stream(k))
+    if rc:
+        check(rc, "kv_cache_append_")
 
 
 def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
@@ -705,42 +770,51 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     included.  ``scale`` defaults to D ** -0.5.  Scores, weights' sums and results are held in fp32; a weight is rounded to the
     values' type before it multiplies them, as the tensor cores take it, and summed as rounded.  Returns [B, T, heads, D].  Pages
     and lengths out of range are raised by ``check_status``."""
-    _half_input(q, "q", 4)
-    k, v, block_table, lengths = _cache_pair(k_cache, v_cache, block_table, lengths, k, v)
+    kind = q.dtype
+    code = _HALF.get(kind)
+    if code is None or q.dim() != 4 or q.get_device() < 0 or (q.requires_grad and torch.is_grad_enabled()):
+        _half_input(q, "q", 4)
+    k, v, new, cache, block_table, lengths = _cache_pair(k_cache, v_cache, block_table, lengths, k, v)
     B, T, H, D = q.shape
-    Hk = k.shape[2]
-    _require(q.dtype == k.dtype and q.device == k.device, "queries must have the keys' dtype and device")
-    _require(k.shape == (B, T, Hk, D), "q must be [B, T, heads, D] and k [B, T, kv_heads, D]")
-    _require(T <= 64, "at most 64 new tokens a sequence")
-    _require(D % 8 == 0 and 0 < D <= 128, "heads must have a multiple of 8 and at most 128 elements")
-    _require(Hk > 0 and H % Hk == 0, "heads must be a multiple of kv_heads")
-    out = torch.empty((B, T, H, D), dtype=q.dtype, device=q.device)
+    Bk, Tk, Hk, Dk = k.shape
+    index = q.get_device()
+    if not (k.dtype is kind and k.get_device() == index and Bk == B and Tk == T and Dk == D and T <= 64 and D % 8 == 0 and 0 < D <= 128
+            and Hk > 0 and H % Hk == 0):
+        _require(kind == k.dtype and q.device == k.device, "queries must have the keys' dtype and device")
+        _require(k.shape == (B, T, Hk, D), "q must be [B, T, heads, D] and k [B, T, kv_heads, D]")
+        _require(T <= 64, "at most 64 new tokens a sequence")
+        _require(D % 8 == 0 and 0 < D <= 128, "heads must have a multiple of 8 and at most 128 elements")
+        _require(False, "heads must be a multiple of kv_heads")
+    out = q.new_empty((B, T, H, D))
     if out.numel() == 0:
         return out
-    mask_ptr = mask_batch = 0
+    mask_at = mask_batch = 0
     if tree_mask is not None:
-        _require(tree_mask.dtype == torch.bool and tree_mask.device == q.device, "tree_mask must be bool, on the queries' device")
-        _require(tree_mask.shape == (B, T, T) or tree_mask.shape == (T, T), "tree_mask must be [B, T, T] or [T, T]")
-        tree_mask = tree_mask.contiguous()
-        mask_ptr, mask_batch = tree_mask.data_ptr(), T * T if tree_mask.dim() == 3 else 0
-    sq = q.stride()
-    if sq[3] != 1 or sq[0] % 2 or sq[1] % 2 or sq[2] % 2 or q.data_ptr() % 4:
+        _require(tree_mask.dtype is torch.bool and tree_mask.get_device() == index, "tree_mask must be bool, on the queries' device")
+        mask_shape = tree_mask.shape
+        _require(mask_shape == (B, T, T) or mask_shape == (T, T), "tree_mask must be [B, T, T] or [T, T]")
+        if not tree_mask.is_contiguous():
+            tree_mask = tree_mask.contiguous()
+        mask_at, mask_batch = tree_mask.data_ptr(), T * T if len(mask_shape) == 3 else 0
+    sq, q_at = q.stride(), q.data_ptr()
+    if sq[3] != 1 or (sq[0] | sq[1] | sq[2]) % 2 or q_at % 4:
         q = q.clone(memory_format=torch.contiguous_format)
-        sq = q.stride()
-    new, cache = k.stride(), k_cache.stride()
-    if new[0] % 8 or new[1] % 8 or new[2] % 8 or k.data_ptr() % 16 or v.data_ptr() % 16:
+        sq, q_at = q.stride(), q.data_ptr()
+    k_at, v_at, k_cache_at, v_cache_at = k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr()
+    if (new[0] | new[1] | new[2]) % 8 or (k_at | v_at) % 16:
         k, v = (t.clone(memory_format=torch.contiguous_format) for t in (k, v))
-        new = k.stride()
-    _require(k_cache.data_ptr() % 16 == 0 and v_cache.data_ptr() % 16 == 0 and cache[0] % 8 == 0 and cache[1] % 8 == 0 and cache[2] % 8 == 0,
-             "cached heads must be 16-byte aligned")
-    dev, width, page = _dev(q), block_table.shape[1], k_cache.shape[1]
-    nbytes = lib.i4tc_tree_attention_scratch_bytes(B, T, H, Hk, D, width * page, dev)
+        new, k_at, v_at = k.stride(), k.data_ptr(), v.data_ptr()
+    _require((k_cache_at | v_cache_at) % 16 == 0 and (cache[0] | cache[1] | cache[2]) % 8 == 0, "cached heads must be 16-byte aligned")
+    pages, page = k_cache.shape[:2]
+    width = block_table.shape[1]
+    nbytes = lib.i4tc_tree_attention_scratch_bytes(B, T, H, Hk, D, width * page, index)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
-    args = _ATTENTION_ARGS.pack(q.data_ptr(), k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(),
-                                lengths.data_ptr(), mask_ptr, out.data_ptr(), scratch.data_ptr(), nbytes, _DTYPES[q.dtype], B, T, H, Hk, D,
-                                k_cache.shape[0], page, width, sq[0], sq[1], sq[2], new[0], new[1], new[2], cache[0], cache[1], cache[2],
-                                block_table.stride(0), mask_batch, D ** -0.5 if scale is None else scale)
-    check(lib.i4tc_tree_attention(args, dev, _stream(q)), "tree_attention")
+    args = _ATTENTION_ARGS.pack(q_at, k_at, v_at, k_cache_at, v_cache_at, block_table.data_ptr(), lengths.data_ptr(), mask_at, out.data_ptr(),
+                                scratch.data_ptr(), nbytes, code, B, T, H, Hk, D, pages, page, width, sq[0], sq[1], sq[2], new[0], new[1], new[2],
+                                cache[0], cache[1], cache[2], block_table.stride(0), mask_batch, D ** -0.5 if scale is None else scale)
+    rc = lib.i4tc_tree_attention(args, index, _raw_stream(index) if _raw_stream is not None else _stream(q))
+    if rc:
+        check(rc, "tree_attention")
     return out
 
 
