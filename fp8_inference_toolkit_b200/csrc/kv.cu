@@ -122,10 +122,11 @@ __device__ __forceinline__ int tiles_of(const AttendParams& p, int length) { ret
 // The line, as a whole warp sees it: its length, and where sequences stand in it (a sequence's tiles come `items` times).  With up to 32
 // sequences a lane keeps its own, so that lengths are read once.
 struct Line {
-  int mine, incl, total;   // of the first 32 sequences: this lane's tiles, and those up to it
+  int length, mine, incl, total;   // of the first 32 sequences: this lane's length and tiles, and the tiles up to it
   __device__ __forceinline__ void open(const AttendParams& p, int items, bool report) {
     const int lane = threadIdx.x & 31;
-    mine = lane < p.batch ? tiles_of(p, cached(p, lane, report)) * items : 0;
+    length = lane < p.batch ? cached(p, lane, report) : 0;
+    mine = lane < p.batch ? tiles_of(p, length) * items : 0;
     incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -140,6 +141,9 @@ struct Line {
       for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
       total += more;
     }
+  }
+  __device__ __forceinline__ int length_of(const AttendParams& p, int b) const {
+    return b < 32 ? __shfl_sync(0xffffffffu, length, b) : b < p.batch ? cached(p, b, false) : 0;
   }
   // Tiles before sequence `upto`.
   __device__ __forceinline__ int before(const AttendParams& p, int items, int upto) const {
@@ -180,17 +184,17 @@ __device__ __forceinline__ int part_of(int total, int parts, int at) { return (i
 // Walks the line tile by tile.
 struct Cursor {
   int b, item, tile, tiles, length;
-  __device__ __forceinline__ void open(const AttendParams& p) {
-    length = b < p.batch ? cached(p, b, false) : 0;
+  __device__ __forceinline__ void open(const AttendParams& p, const Line& line) {
+    length = line.length_of(p, b);
     tiles = tiles_of(p, length);
   }
-  __device__ __forceinline__ void next(const AttendParams& p) {
+  __device__ __forceinline__ void next(const AttendParams& p, const Line& line) {
     if (++tile < tiles) return;
     tile = 0;
     if (++item < p.kv_heads * p.row_tiles) return;
     item = 0;
     ++b;
-    open(p);
+    open(p, line);
   }
 };
 
@@ -285,18 +289,18 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
   Cursor cur;
   int before;
   cur.b = line.find(p, items, first, before);
-  cur.open(p);
+  cur.open(p, line);
   cur.item = (first - before) / cur.tiles;
   cur.tile = (first - before) % cur.tiles;
   Cursor ahead = cur;                               // whose places are looked up next
 
   // Places of the tile at `ahead`: key tid of it.  In two halves, the page's number and the addresses, so that nobody waits for the table.
   // Where there is no place (behind the new tokens, pages out of range) some row that exists.
-  auto look_up = [&]() -> int {
+  auto look_up = [&](const Cursor& ahead) -> int {
     const int j = ahead.tile * kTile + tid;
     return j < ahead.length ? __ldg(p.table + ahead.b * p.table_stride + j / p.page_size) : 0;
   };
-  auto place_of = [&](int page) -> ulonglong2 {
+  auto place_of = [&](const Cursor& ahead, int page) -> ulonglong2 {
     const int j = ahead.tile * kTile + tid, head = ahead.item / p.row_tiles;
     const char *k = static_cast<const char*>(p.k), *v = static_cast<const char*>(p.v);
     long long at = ahead.b * p.new_batch + min(max(j - ahead.length, 0), p.tokens - 1) * p.new_token + head * p.new_head;
@@ -329,15 +333,21 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
       cp_async_16(dk + S::kStage + r * (DP * 2), pv, n);
     }
   };
-  int rows[kStages];                                // of the tiles ahead: keys that exist
+  int rows[kStages], pages[kStages];                // of the tiles ahead: keys that exist, and this thread's page
+  Cursor at[kStages];
 #pragma unroll
   for (int i = 0; i < kStages; ++i) {
+    at[i] = ahead;
     rows[i] = ahead.length + p.tokens - ahead.tile * kTile;
+    pages[i] = 0;
     if (i < count) {
-      if (tid < kTile) places[i * kTile + tid] = place_of(look_up());
-      ahead.next(p);
+      if (tid < kTile) pages[i] = look_up(ahead);
+      ahead.next(p, line);
     }
   }
+#pragma unroll
+  for (int i = 0; i < kStages; ++i)
+    if (i < count && tid < kTile) places[i * kTile + tid] = place_of(at[i], pages[i]);
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kStages - 1; ++i) {
@@ -359,8 +369,33 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
     k_at[j] = stage0 + kr * (DP * 2) + (((2 * j + ((lane >> 3) & 1)) ^ (kr & 7)) * 16);
     v_at[j] = stage0 + S::kStage + vr * (DP * 2) + (((2 * j + (lane >> 4)) ^ (vr & 7)) * 16);
   }
-  bool begun = true, whole = cur.tile == 0;         // begun: the item's rows have to be set up; whole: this part has it from its start
+  bool whole = cur.tile == 0;                       // this part has the item from its start
 
+  // The item's queries and running state.
+  auto begin = [&]() {
+    const int row0 = (cur.item % p.row_tiles) * S::ROWS + wr * 16 + g, kvh = cur.item / p.row_tiles;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = row0 + 8 * h;
+      tok[h] = row < p.rows ? row / p.group : -1;
+      const T* src = static_cast<const T*>(p.q) + cur.b * p.q_batch + (long long)(row / p.group) * p.q_token +
+                     (long long)(kvh * p.group + row % p.group) * p.q_head;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int d = ks * 16 + e * 8 + 2 * t4;
+          q[ks][2 * e + h] = tok[h] >= 0 && d < p.D ? *reinterpret_cast<const uint32_t*>(src + d) ^ p.flip : 0u;
+        }
+      m[h] = -CUDART_INF_F;
+      l[2 * h] = l[2 * h + 1] = 0.f;
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[dt][k] = 0.f;
+  };
+  begin();                                          // (its loads under the first tiles' copies)
   int stage = 0;                                    // of tile i
   for (int i = 0; i < count; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
@@ -369,33 +404,8 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
     asm volatile("cp.async.commit_group;" ::: "memory");
     const bool more = i + kStages < count;
     int page = 0;
-    if (more && tid < kTile) page = look_up();
+    if (more && tid < kTile) page = look_up(ahead);
     next_rows = ahead.length + p.tokens - ahead.tile * kTile;
-
-    if (begun) {
-      const int row0 = (cur.item % p.row_tiles) * S::ROWS + wr * 16 + g, kvh = cur.item / p.row_tiles;
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int row = row0 + 8 * h;
-        tok[h] = row < p.rows ? row / p.group : -1;
-        const T* src = static_cast<const T*>(p.q) + cur.b * p.q_batch + (long long)(row / p.group) * p.q_token +
-                       (long long)(kvh * p.group + row % p.group) * p.q_head;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int d = ks * 16 + e * 8 + 2 * t4;
-            q[ks][2 * e + h] = tok[h] >= 0 && d < p.D ? *reinterpret_cast<const uint32_t*>(src + d) ^ p.flip : 0u;
-          }
-        m[h] = -CUDART_INF_F;
-        l[2 * h] = l[2 * h + 1] = 0.f;
-      }
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) o[dt][k] = 0.f;
-      begun = false;
-    }
 
     const uint32_t at_stage = stage * 2 * S::kStage, sv = stage0 + at_stage + S::kStage;
     if (++stage == kStages) stage = 0;
@@ -601,12 +611,14 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
           }
         }
       }
-      begun = whole = true;
+      whole = true;
     }
-    cur.next(p);
+    const bool another = ends && i + 1 < count;
+    cur.next(p, line);
+    if (another) begin();
     if (more) {
-      if (tid < kTile) places[((i + kStages) % kPlaces) * kTile + tid] = place_of(page);
-      ahead.next(p);
+      if (tid < kTile) places[((i + kStages) % kPlaces) * kTile + tid] = place_of(ahead, page);
+      ahead.next(p, line);
     }
   }
 }
@@ -617,43 +629,67 @@ template <typename T, int DP>
 __global__ void __launch_bounds__(kAttendThreads) attend_join_kernel(const AttendParams p, int tile_rows) {
   constexpr int E = DP / 32, WARPS = kAttendThreads / 32;
   __shared__ float sums[WARPS][DP + 2];
-  pdl_wait();
+  // The lengths may be read before the wait: the kernel before this one let it start after its own wait, and writes scratch and results only.
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int items = p.kv_heads * p.row_tiles;
   const int b = blockIdx.x / items, item = blockIdx.x % items, row = blockIdx.y;
   const int at_row = (item % p.row_tiles) * tile_rows + row;
-  if (at_row >= p.rows) return;
   Line line;
   line.open(p, items, false);
-  const int length = cached(p, b, false), tiles = tiles_of(p, length);
+  const int length = line.length_of(p, b), tiles = tiles_of(p, length);
   const int start = line.before(p, items, b) + item * tiles;
   const int parts = min(p.parts, line.total);
   const int first = part_of(line.total, parts, start), last = part_of(line.total, parts, start + tiles - 1);
-  if (first == last) return;
   const size_t step = 2 * slot_floats(tile_rows, DP);
-  const float* opening = p.scratch + first * step + (part_start(line.total, parts, first) == start ? 0 : step / 2);
-  auto slot = [&](int part) { return part == first ? opening : p.scratch + part * step; };
+  const bool begins = part_start(line.total, parts, first) == start;
+  pdl_wait();
+  if (at_row >= p.rows || first == last) return;
+  const float* scratch = p.scratch;
+  pdl_fresh(scratch);
+  const float* opening = scratch + first * step + (begins ? 0 : step / 2);
+  auto slot = [&](int part) { return part == first ? opening : scratch + part * step; };
   const int count = last - first + 1, each = (count + WARPS - 1) / WARPS;
   const int from = first + min(count, warp * each), to = first + min(count, (warp + 1) * each);
   float top = -CUDART_INF_F, sum = 0.f, v[E];
-  for (int part = from + lane; part < to; part += 32) top = fmaxf(top, slot(part)[row]);
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float zero = top == -CUDART_INF_F ? 0.f : top;
 #pragma unroll
   for (int e = 0; e < E; ++e) v[e] = 0.f;
-#pragma unroll 8
-  for (int part = from; part < to; ++part) {
-    const float* s = slot(part);
-    const float f = exp2_fast(s[row] - zero);
-    sum += s[tile_rows + row] * f;
-    const float* o = s + 2 * tile_rows + row * DP + lane * E;
-    if constexpr (E == 4) {
-      const float4 x = *reinterpret_cast<const float4*>(o);
-      v[0] += x.x * f; v[1] += x.y * f; v[2] += x.z * f; v[3] += x.w * f;
-    } else {
-      const float2 x = *reinterpret_cast<const float2*>(o);
-      v[0] += x.x * f; v[1] += x.y * f;
+  constexpr int AT_ONCE = 8;                        // parts whose loads are on their way together
+  for (int part = from; part < to; part += AT_ONCE) {
+    float m[AT_ONCE], l[AT_ONCE], x[AT_ONCE][E];
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      m[k] = -CUDART_INF_F;
+      l[k] = 0.f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) x[k][e] = 0.f;
+      if (part + k < to) {
+        const float* s = slot(part + k);
+        m[k] = s[row];
+        l[k] = s[tile_rows + row];
+        const float* o = s + 2 * tile_rows + row * DP + lane * E;
+        if constexpr (E == 4) {
+          const float4 q = *reinterpret_cast<const float4*>(o);
+          x[k][0] = q.x; x[k][1] = q.y; x[k][2] = q.z; x[k][3] = q.w;
+        } else {
+          const float2 q = *reinterpret_cast<const float2*>(o);
+          x[k][0] = q.x; x[k][1] = q.y;
+        }
+      }
+    }
+    float both = top;
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) both = fmaxf(both, m[k]);
+    const float zero = both == -CUDART_INF_F ? 0.f : both, fade = exp2_fast(top - zero);
+    top = both;
+    sum *= fade;
+#pragma unroll
+    for (int e = 0; e < E; ++e) v[e] *= fade;
+#pragma unroll
+    for (int k = 0; k < AT_ONCE; ++k) {
+      const float f = exp2_fast(m[k] - zero);
+      sum += l[k] * f;
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] += x[k][e] * f;
     }
   }
 #pragma unroll
