@@ -82,11 +82,11 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
 // key's 2 D bytes serve T * group rows (64 at sixteen drafts of four heads: 64 operations a byte, below what mma.sync gives; a
 // tcgen05 tile of 128 rows would be padding for nearly all trees).  One pass with the running maximum and sum of the softmax.
 //
-// The work is 64-key tiles.  The tiles of all sequences, heads and row tiles stand in one line, which is cut into equal parts,
-// one a block: ragged lengths, one long sequence and many short ones all keep every block busy alike.  A part begins and
-// ends anywhere; what it holds of an item (sequence, kv head, row tile) goes out as the result where it holds all of it, else
-// as maximum, sum and weighted values (fp32) to scratch, and a second kernel adds an item's parts in ascending order.  No
-// atomics: the same bits in every run.
+// The work is 64-key tiles.  The tiles of all sequences stand in one line, which is cut into equal parts, and every (kv head, row tile) has
+// a block for each part: ragged lengths, one long sequence and many short ones all keep every block busy alike, and the heads of
+// a token, side by side in a page, are read at the same time.  A part begins and ends anywhere; what it holds of a sequence goes out
+// as the result where it holds all of it, else as maximum, sum and weighted values (fp32) to scratch, and a second kernel adds a
+// sequence's parts in ascending order.  No atomics: the same bits in every run.
 //
 // A block's four warps are WR row warps (16 rows each) times 4 / WR key warps, which share out a tile's keys and are added at the
 // item's end: few rows do not leave warps idle.  Tiles arrive by cp.async, two ahead; a key's address (its page) is looked
@@ -104,7 +104,8 @@ struct AttendParams {
   int batch, tokens, heads, kv_heads, group, D;
   int pages, page_size, table_width;
   int rows, row_tiles;          // of an item: tokens * group
-  int parts;                    // blocks
+  int lines;                    // kv heads times row tiles: blocks of a part
+  int parts;                    // of the line, at most
   float scale_log2;             // |scale| * log2(e), not zero: what is masked stays so
   uint32_t flip;                // sign bits of two queries, where the scale is negative
   unsigned int* status;
@@ -119,14 +120,14 @@ __device__ __forceinline__ int cached(const AttendParams& p, int b, bool report)
 }
 __device__ __forceinline__ int tiles_of(const AttendParams& p, int length) { return (length + p.tokens + kTile - 1) / kTile; }
 
-// The line, as a whole warp sees it: its length, and where sequences stand in it (a sequence's tiles come `items` times).  With up to 32
+// The line, as a whole warp sees it: its length, and where sequences stand in it.  With up to 32
 // sequences a lane keeps its own, so that lengths are read once.
 struct Line {
   int length, mine, incl, total;   // of the first 32 sequences: this lane's length and tiles, and the tiles up to it
-  __device__ __forceinline__ void open(const AttendParams& p, int items, bool report) {
+  __device__ __forceinline__ void open(const AttendParams& p, bool report) {
     const int lane = threadIdx.x & 31;
     length = lane < p.batch ? cached(p, lane, report) : 0;
-    mine = lane < p.batch ? tiles_of(p, length) * items : 0;
+    mine = lane < p.batch ? tiles_of(p, length) : 0;
     incl = mine;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -136,7 +137,7 @@ struct Line {
     total = __shfl_sync(0xffffffffu, incl, 31);
     if (p.batch > 32) {
       int more = 0;
-      for (int b = 32 + lane; b < p.batch; b += 32) more += tiles_of(p, cached(p, b, report)) * items;
+      for (int b = 32 + lane; b < p.batch; b += 32) more += tiles_of(p, cached(p, b, report));
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
       total += more;
@@ -146,16 +147,16 @@ struct Line {
     return b < 32 ? __shfl_sync(0xffffffffu, length, b) : b < p.batch ? cached(p, b, false) : 0;
   }
   // Tiles before sequence `upto`.
-  __device__ __forceinline__ int before(const AttendParams& p, int items, int upto) const {
+  __device__ __forceinline__ int before(const AttendParams& p, int upto) const {
     if (upto < 32) return __shfl_sync(0xffffffffu, incl - mine, upto);
     int more = 0;
-    for (int b = 32 + (threadIdx.x & 31); b < upto; b += 32) more += tiles_of(p, cached(p, b, false)) * items;
+    for (int b = 32 + (threadIdx.x & 31); b < upto; b += 32) more += tiles_of(p, cached(p, b, false));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) more += __shfl_xor_sync(0xffffffffu, more, o);
     return more + __shfl_sync(0xffffffffu, incl, 31);
   }
   // The sequence that holds tile `at`, and the tiles before it.
-  __device__ __forceinline__ int find(const AttendParams& p, int items, int at, int& start) const {
+  __device__ __forceinline__ int find(const AttendParams& p, int at, int& start) const {
     int b0 = 0, base = 0, m = mine, upto = incl;
     for (;;) {
       const unsigned past = __ballot_sync(0xffffffffu, base + upto > at);
@@ -167,7 +168,7 @@ struct Line {
       base += __shfl_sync(0xffffffffu, upto, 31);
       b0 += 32;
       const int lane = threadIdx.x & 31;
-      m = b0 + lane < p.batch ? tiles_of(p, cached(p, b0 + lane, false)) * items : 0;
+      m = b0 + lane < p.batch ? tiles_of(p, cached(p, b0 + lane, false)) : 0;
       upto = m;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -183,7 +184,7 @@ __device__ __forceinline__ int part_of(int total, int parts, int at) { return (i
 
 // Walks the line tile by tile.
 struct Cursor {
-  int b, item, tile, tiles, length;
+  int b, tile, tiles, length;
   __device__ __forceinline__ void open(const AttendParams& p, const Line& line) {
     length = line.length_of(p, b);
     tiles = tiles_of(p, length);
@@ -191,8 +192,6 @@ struct Cursor {
   __device__ __forceinline__ void next(const AttendParams& p, const Line& line) {
     if (++tile < tiles) return;
     tile = 0;
-    if (++item < p.kv_heads * p.row_tiles) return;
-    item = 0;
     ++b;
     open(p, line);
   }
@@ -280,18 +279,17 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
   pdl_wait();
   pdl_trigger();
 
-  const int items = p.kv_heads * p.row_tiles;
+  const int part = blockIdx.x / p.lines, kvh = blockIdx.x % p.lines / p.row_tiles, tile_row0 = blockIdx.x % p.lines % p.row_tiles * S::ROWS;
   Line line;
-  line.open(p, items, blockIdx.x == 0);
-  const int parts = min(p.parts, line.total), part = blockIdx.x;   // no part is empty
+  line.open(p, blockIdx.x == 0);
+  const int parts = min(p.parts, line.total);       // no part is empty
   if (part >= parts) return;
   const int first = part_start(line.total, parts, part), count = part_start(line.total, parts, part + 1) - first;
   Cursor cur;
   int before;
-  cur.b = line.find(p, items, first, before);
+  cur.b = line.find(p, first, before);
   cur.open(p, line);
-  cur.item = (first - before) / cur.tiles;
-  cur.tile = (first - before) % cur.tiles;
+  cur.tile = first - before;
   Cursor ahead = cur;                               // whose places are looked up next
 
   // Places of the tile at `ahead`: key tid of it.  In two halves, the page's number and the addresses, so that nobody waits for the table.
@@ -301,12 +299,12 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
     return j < ahead.length ? __ldg(p.table + ahead.b * p.table_stride + j / p.page_size) : 0;
   };
   auto place_of = [&](const Cursor& ahead, int page) -> ulonglong2 {
-    const int j = ahead.tile * kTile + tid, head = ahead.item / p.row_tiles;
+    const int j = ahead.tile * kTile + tid;
     const char *k = static_cast<const char*>(p.k), *v = static_cast<const char*>(p.v);
-    long long at = ahead.b * p.new_batch + min(max(j - ahead.length, 0), p.tokens - 1) * p.new_token + head * p.new_head;
+    long long at = ahead.b * p.new_batch + min(max(j - ahead.length, 0), p.tokens - 1) * p.new_token + kvh * p.new_head;
     if (j < ahead.length) {
       if (page >= 0 && page < p.pages) {
-        at = page * p.page_stride + (j % p.page_size) * p.slot_stride + head * p.head_stride;
+        at = page * p.page_stride + (j % p.page_size) * p.slot_stride + kvh * p.head_stride;
         k = static_cast<const char*>(p.k_cache);
         v = static_cast<const char*>(p.v_cache);
       } else {
@@ -373,7 +371,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
 
   // The item's queries and running state.
   auto begin = [&]() {
-    const int row0 = (cur.item % p.row_tiles) * S::ROWS + wr * 16 + g, kvh = cur.item / p.row_tiles;
+    const int row0 = tile_row0 + wr * 16 + g;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const int row = row0 + 8 * h;
@@ -427,40 +425,46 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
     const bool edge = j0 + kTile > cur.length;      // the tile holds new tokens, or what is behind them
     bool odd = false;
     if (edge) {
-      // not only the scores of what a row does not see: its values may be infinite or no numbers, which a weight of zero does not undo
+      // Which of this lane's keys its two rows see, as bits: the cached ones, then the row's bits of the mask (four lanes have a row and
+      // read a quarter of them each).  Rolled, as is the next loop: an item comes here once, and what it does not run it need not fetch.
+      const int rel = cur.length - (j0 + key0 + 2 * t4);
+      uint64_t seen[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        uint64_t bits = 0;
+        if (tok[h] >= 0) {
+          if (p.mask == nullptr) {
+            bits = ~0ull >> (63 - tok[h]);
+          } else {
+            const uint8_t* row = p.mask + cur.b * p.mask_batch + (long long)tok[h] * p.tokens;
+#pragma unroll 2
+            for (int j = t4; j < p.tokens; j += 4) bits |= (uint64_t)(row[j] != 0) << j;
+          }
+        }
+        bits |= __shfl_xor_sync(0xffffffffu, bits, 1);
+        bits |= __shfl_xor_sync(0xffffffffu, bits, 2);
+        seen[h] = rel >= 64 ? ~0ull : rel > 0 ? bits << rel | ((1ull << rel) - 1) : rel > -64 ? bits >> -rel : 0ull;
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          if (!(seen[k >> 1] >> (nt * 8 + (k & 1)) & 1)) s[nt][k] = -CUDART_INF_F;
+      // Not only the scores of what a row does not see: its values may be infinite or no numbers, which a weight of zero does not undo.
+#pragma unroll 1
       for (int r = tid; r < kTile * CH; r += kAttendThreads) {
         const int key = r / CH, c = r % CH;
         if (j0 + key < cur.length) continue;
         const uint32_t at = sv + key * (DP * 2) + ((c ^ (key & 7)) * 16);
+        constexpr uint32_t kExp = std::is_same_v<T, __half> ? 0x7C007C00u : 0x7F807F80u;
         uint4 v = ptx::lds128(at);
-        uint32_t* u = &v.x;
-        bool hit = false;
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            constexpr uint32_t kExp = std::is_same_v<T, __half> ? 0x7C00u : 0x7F80u;
-            if (((u[k] >> (16 * half)) & kExp) == kExp) {
-              u[k] &= half ? 0x0000FFFFu : 0xFFFF0000u;
-              hit = true;
-            }
-          }
-        if (hit) {
-          ptx::sts128(at, v);
+        const uint32_t x = __vcmpeq2(v.x & kExp, kExp), y = __vcmpeq2(v.y & kExp, kExp), z = __vcmpeq2(v.z & kExp, kExp), w = __vcmpeq2(v.w & kExp, kExp);
+        if (x | y | z | w) {
+          ptx::sts128(at, make_uint4(v.x & ~x, v.y & ~y, v.z & ~z, v.w & ~w));
           odd = true;
         }
       }
       odd = __syncthreads_or(odd);
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const int j = j0 + key0 + nt * 8 + 2 * t4 + (k & 1) - cur.length, t = tok[k >> 1];
-          bool seen = j < 0;
-          if (j >= 0 && j < p.tokens && t >= 0)
-            seen = p.mask ? p.mask[cur.b * p.mask_batch + (long long)t * p.tokens + j] != 0 : j <= t;
-          if (!seen) s[nt][k] = -CUDART_INF_F;
-        }
     }
 
     float top[2] = {m[0], m[1]};
@@ -492,24 +496,24 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
 #pragma unroll
     for (int h = 0; h < 2; ++h) base[h] = m[h] == -CUDART_INF_F ? 0.f : m[h] * p.scale_log2 - kLift;
     if (odd) {                                      // what was taken out of the values goes to the rows that see it
+#pragma unroll 1
       for (int key = key0; key < key0 + S::KEYS; ++key) {
         const int j = j0 + key - cur.length;
         if (j < 0 || j >= p.tokens) continue;
-        const T* src = static_cast<const T*>(p.v) + cur.b * p.new_batch + j * p.new_token + (long long)(cur.item / p.row_tiles) * p.new_head;
+        const T* src = static_cast<const T*>(p.v) + cur.b * p.new_batch + j * p.new_token + kvh * p.new_head;
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
           const int t = tok[h];
           if (t < 0 || !(p.mask ? p.mask[cur.b * p.mask_batch + (long long)t * p.tokens + j] != 0 : j <= t)) continue;
 #pragma unroll
-          for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int d = dt * 8 + 2 * t4 + e;
-              if (d < p.D) {
-                const float x = to_f32(src[d]);
-                if (!isfinite(x)) o[dt][2 * h + e] += x;
-              }
+          for (int dt = 0; dt < DT; ++dt) {
+            const int d = dt * 8 + 2 * t4;
+            if (d < p.D) {
+              const float x = to_f32(src[d]), y = to_f32(src[d + 1]);
+              if (!isfinite(x)) o[dt][2 * h] += x;
+              if (!isfinite(y)) o[dt][2 * h + 1] += y;
             }
+          }
         }
       }
     }
@@ -540,6 +544,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
         // the key warps, one after the other and half of the elements at a time, into the first
         float* mo = merge + (wr * 16 + g) * (DP / 2) + 2 * t4;
         float* ml = merge + S::ROWS * (DP / 2) + (wr * 16 + g) * 2;
+#pragma unroll 1
         for (int from = 1; from < S::WK; ++from) {
           float fa[2], fb[2];
 #pragma unroll
@@ -580,7 +585,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
         }
       }
       if (wk == 0) {
-        const int row0 = (cur.item % p.row_tiles) * S::ROWS + wr * 16 + g, kvh = cur.item / p.row_tiles;
+        const int row0 = tile_row0 + wr * 16 + g;
         if (whole && ends) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -597,7 +602,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
         } else {
           // the item the part began in, or (where that is another) the one it ends in
           const bool opening = !whole || i == cur.tile;
-          float* slot = p.scratch + ((size_t)part * 2 + (opening ? 0 : 1)) * slot_floats(S::ROWS, DP);
+          float* slot = p.scratch + ((size_t)blockIdx.x * 2 + (opening ? 0 : 1)) * slot_floats(S::ROWS, DP);
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int row = wr * 16 + g + 8 * h;
@@ -631,22 +636,22 @@ __global__ void __launch_bounds__(kAttendThreads) attend_join_kernel(const Atten
   __shared__ float sums[WARPS][DP + 2];
   // The lengths may be read before the wait: the kernel before this one let it start after its own wait, and writes scratch and results only.
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int items = p.kv_heads * p.row_tiles;
-  const int b = blockIdx.x / items, item = blockIdx.x % items, row = blockIdx.y;
-  const int at_row = (item % p.row_tiles) * tile_rows + row;
+  const int b = blockIdx.x / p.lines, at_line = blockIdx.x % p.lines, row = blockIdx.y;
+  const int at_row = at_line % p.row_tiles * tile_rows + row;
   Line line;
-  line.open(p, items, false);
+  line.open(p, false);
   const int length = line.length_of(p, b), tiles = tiles_of(p, length);
-  const int start = line.before(p, items, b) + item * tiles;
+  const int start = line.before(p, b);
   const int parts = min(p.parts, line.total);
   const int first = part_of(line.total, parts, start), last = part_of(line.total, parts, start + tiles - 1);
-  const size_t step = 2 * slot_floats(tile_rows, DP);
+  const size_t slots = 2 * slot_floats(tile_rows, DP), step = slots * p.lines;   // a block's, and from a part to the next
   const bool begins = part_start(line.total, parts, first) == start;
   pdl_wait();
   if (at_row >= p.rows || first == last) return;
   const float* scratch = p.scratch;
   pdl_fresh(scratch);
-  const float* opening = scratch + first * step + (begins ? 0 : step / 2);
+  scratch += at_line * slots;
+  const float* opening = scratch + first * step + (begins ? 0 : slots / 2);
   auto slot = [&](int part) { return part == first ? opening : scratch + part * step; };
   const int count = last - first + 1, each = (count + WARPS - 1) / WARPS;
   const int from = first + min(count, warp * each), to = first + min(count, (warp + 1) * each);
@@ -712,7 +717,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_join_kernel(const Atten
     sum += sums[k][DP + 1] * f;
     if (d < DP) x += sums[k][d] * f;
   }
-  const int t = at_row / p.group, head = (item / p.row_tiles) * p.group + at_row % p.group;
+  const int t = at_row / p.group, head = at_line / p.row_tiles * p.group + at_row % p.group;
   if (d < p.D) {
     const float y = x * inverse_sum(p, sum, b, t, length);
     T* dst = static_cast<T*>(p.out) + (((long long)b * p.tokens + t) * p.heads + head) * p.D + d;
@@ -722,9 +727,10 @@ __global__ void __launch_bounds__(kAttendThreads) attend_join_kernel(const Atten
 
 int row_warps(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 int padded_dim(int64_t D) { return D <= 64 ? 64 : 128; }
-int attend_parts(int sm_count, int64_t batch, int64_t items, int64_t most_length, int64_t tokens) {
-  const int64_t tiles = batch * items * ((most_length + tokens + kTile - 1) / kTile), most = (int64_t)sm_count * 2;
-  return (int)(tiles < most ? tiles : most);
+// Parts of the line: two blocks an SM in all.
+int attend_parts(int sm_count, int64_t batch, int64_t lines, int64_t most_length, int64_t tokens) {
+  const int64_t tiles = batch * ((most_length + tokens + kTile - 1) / kTile), most = (int64_t)sm_count * 2 / lines;
+  return (int)(most < 1 ? 1 : tiles < most ? tiles : most);
 }
 
 template <typename T, int DP, int WR>
@@ -738,8 +744,8 @@ int launch_attend(const AttendParams& p, cudaStream_t st) {
     I4TC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     if (dev < 64) configured[dev] = true;
   }
-  I4TC_CUDA(launch_kernel(true, kernel, dim3((unsigned)p.parts), kAttendThreads, S::kSmem, st, p));
-  const dim3 grid((unsigned)(p.batch * p.kv_heads * p.row_tiles), (unsigned)(S::ROWS < p.rows ? S::ROWS : p.rows));
+  I4TC_CUDA(launch_kernel(true, kernel, dim3((unsigned)(p.parts * p.lines)), kAttendThreads, S::kSmem, st, p));
+  const dim3 grid((unsigned)(p.batch * p.lines), (unsigned)(S::ROWS < p.rows ? S::ROWS : p.rows));
   I4TC_CUDA(launch_kernel(true, attend_join_kernel<T, DP>, grid, kAttendThreads, 0, st, p, S::ROWS));
   return I4TC_OK;
 }
@@ -760,8 +766,8 @@ extern "C" int64_t i4tc_tree_attention_scratch_bytes(int64_t batch, int64_t toke
   if (batch <= 0 || tokens <= 0 || heads <= 0 || kv_heads <= 0 || D <= 0 || most_length < 0 || device_info(device, &info) != I4TC_OK) return 0;
   const int64_t rows = tokens * (heads / kv_heads);
   const int tile_rows = 16 * row_warps(rows);
-  const int64_t items = kv_heads * ((rows + tile_rows - 1) / tile_rows);
-  return (int64_t)attend_parts(info->sm_count, batch, items, most_length, tokens) * 2 * (int64_t)slot_floats(tile_rows, padded_dim(D)) * 4;
+  const int64_t lines = kv_heads * ((rows + tile_rows - 1) / tile_rows);
+  return attend_parts(info->sm_count, batch, lines, most_length, tokens) * lines * 2 * (int64_t)slot_floats(tile_rows, padded_dim(D)) * 4;
 }
 
 extern "C" int i4tc_tree_attention(const i4tc_tree_attention_args* a, int device, void* stream) {
@@ -797,12 +803,13 @@ extern "C" int i4tc_tree_attention(const i4tc_tree_attention_args* a, int device
   const int64_t rows = (int64_t)p.tokens * p.group;
   const int warps = row_warps(rows);
   p.rows = (int)rows; p.row_tiles = (int)((rows + 16 * warps - 1) / (16 * warps));
-  const int64_t items = (int64_t)p.kv_heads * p.row_tiles;
+  p.lines = p.kv_heads * p.row_tiles;
   const int64_t most_length = a->table_width * a->page_size;
-  I4TC_REQUIRE(most_length < (1ll << 31) - 2 * kTile && a->batch * items * ((most_length + a->tokens) / kTile + 1) < (1ll << 31), I4TC_EUNSUPPORTED,
-               "the table has room for too many tokens");
-  p.parts = attend_parts(info->sm_count, a->batch, items, most_length, a->tokens);
-  I4TC_REQUIRE(a->scratch_bytes >= (int64_t)p.parts * 2 * (int64_t)slot_floats(16 * warps, padded_dim(p.D)) * 4, I4TC_EWORKSPACE, "the scratch is too small");
+  I4TC_REQUIRE(most_length < (1ll << 31) - 2 * kTile && a->batch * ((most_length + a->tokens) / kTile + 1) < (1ll << 31) && a->batch * p.lines < (1ll << 31),
+               I4TC_EUNSUPPORTED, "the table has room for too many tokens");
+  p.parts = attend_parts(info->sm_count, a->batch, p.lines, most_length, a->tokens);
+  I4TC_REQUIRE(a->scratch_bytes >= (int64_t)p.parts * p.lines * 2 * (int64_t)slot_floats(16 * warps, padded_dim(p.D)) * 4, I4TC_EWORKSPACE,
+               "the scratch is too small");
   p.scale_log2 = fmaxf((float)(fabs(a->scale) * 1.4426950408889634), 1e-30f);
   p.flip = a->scale < 0 ? 0x80008000u : 0u;
   p.status = info->status;
