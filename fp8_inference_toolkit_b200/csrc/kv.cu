@@ -91,7 +91,7 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
 // A block's four warps are WR row warps (16 rows each) times 4 / WR key warps, which share out a tile's keys and are added at the
 // item's end: few rows do not leave warps idle.  Tiles arrive by cp.async, two ahead; a key's address (its page) is looked
 // up one tile before that.
-constexpr int kTile = 64, kStages = 3, kAttendThreads = 128, kPlaces = 4;
+constexpr int kTile = 64, kStages = 3, kAttendThreads = 128, kPlaces = 4, kJoinThreads = 128;
 
 struct AttendParams {
   const void *q, *k, *v, *k_cache, *v_cache;
@@ -628,16 +628,16 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
   }
 }
 
-// Items that no part held whole: their parts in ascending order.  A block takes a row: its warps a quarter of the parts each, which are
-// added in order in the end; a lane DP / 32 consecutive elements.
+// Sequences that no part held whole: their parts in ascending order.  A block takes rows_each rows of a (sequence, line).  Few parts: a warp
+// has a row to itself.  More: the block's warps take a quarter of the parts each, and these are added in order.  A lane has DP / 32
+// consecutive elements.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kAttendThreads) attend_join_kernel(const AttendParams p, int tile_rows) {
-  constexpr int E = DP / 32, WARPS = kAttendThreads / 32;
+__global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const AttendParams p, int tile_rows, int rows_each) {
+  constexpr int E = DP / 32, WARPS = kJoinThreads / 32, AT_ONCE = 8;   // AT_ONCE: parts whose loads are on their way together
   __shared__ float sums[WARPS][DP + 2];
   // The lengths may be read before the wait: the kernel before this one let it start after its own wait, and writes scratch and results only.
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int b = blockIdx.x / p.lines, at_line = blockIdx.x % p.lines, row = blockIdx.y;
-  const int at_row = at_line % p.row_tiles * tile_rows + row;
+  const int b = blockIdx.x / p.lines, at_line = blockIdx.x % p.lines, row0 = blockIdx.y * rows_each;
   Line line;
   line.open(p, false);
   const int length = line.length_of(p, b), tiles = tiles_of(p, length);
@@ -647,81 +647,105 @@ __global__ void __launch_bounds__(kAttendThreads) attend_join_kernel(const Atten
   const size_t slots = 2 * slot_floats(tile_rows, DP), step = slots * p.lines;   // a block's, and from a part to the next
   const bool begins = part_start(line.total, parts, first) == start;
   pdl_wait();
-  if (at_row >= p.rows || first == last) return;
+  const int rows = min(rows_each, min(tile_rows, p.rows - at_line % p.row_tiles * tile_rows) - row0);
+  if (rows <= 0 || first == last) return;
   const float* scratch = p.scratch;
   pdl_fresh(scratch);
   scratch += at_line * slots;
   const float* opening = scratch + first * step + (begins ? 0 : slots / 2);
   auto slot = [&](int part) { return part == first ? opening : scratch + part * step; };
-  const int count = last - first + 1, each = (count + WARPS - 1) / WARPS;
-  const int from = first + min(count, warp * each), to = first + min(count, (warp + 1) * each);
-  float top = -CUDART_INF_F, sum = 0.f, v[E];
+  float top, sum, v[E];
+  auto gather = [&](int row, int from, int to) {    // parts [from, to) of a row into top, sum and v
+    top = -CUDART_INF_F;
+    sum = 0.f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) v[e] = 0.f;
-  constexpr int AT_ONCE = 8;                        // parts whose loads are on their way together
-  for (int part = from; part < to; part += AT_ONCE) {
-    float m[AT_ONCE], l[AT_ONCE], x[AT_ONCE][E];
+    for (int e = 0; e < E; ++e) v[e] = 0.f;
+    for (int part = from; part < to; part += AT_ONCE) {
+      float m[AT_ONCE], l[AT_ONCE], x[AT_ONCE][E];
 #pragma unroll
-    for (int k = 0; k < AT_ONCE; ++k) {
-      m[k] = -CUDART_INF_F;
-      l[k] = 0.f;
+      for (int k = 0; k < AT_ONCE; ++k) {
+        m[k] = -CUDART_INF_F;
+        l[k] = 0.f;
 #pragma unroll
-      for (int e = 0; e < E; ++e) x[k][e] = 0.f;
-      if (part + k < to) {
-        const float* s = slot(part + k);
-        m[k] = s[row];
-        l[k] = s[tile_rows + row];
-        const float* o = s + 2 * tile_rows + row * DP + lane * E;
-        if constexpr (E == 4) {
-          const float4 q = *reinterpret_cast<const float4*>(o);
-          x[k][0] = q.x; x[k][1] = q.y; x[k][2] = q.z; x[k][3] = q.w;
-        } else {
-          const float2 q = *reinterpret_cast<const float2*>(o);
-          x[k][0] = q.x; x[k][1] = q.y;
+        for (int e = 0; e < E; ++e) x[k][e] = 0.f;
+        if (part + k < to) {
+          const float* s = slot(part + k);
+          m[k] = s[row];
+          l[k] = s[tile_rows + row];
+          const float* o = s + 2 * tile_rows + row * DP + lane * E;
+          if constexpr (E == 4) {
+            const float4 q = *reinterpret_cast<const float4*>(o);
+            x[k][0] = q.x; x[k][1] = q.y; x[k][2] = q.z; x[k][3] = q.w;
+          } else {
+            const float2 q = *reinterpret_cast<const float2*>(o);
+            x[k][0] = q.x; x[k][1] = q.y;
+          }
         }
       }
+      float both = top;
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) both = fmaxf(both, m[k]);
+      const float zero = both == -CUDART_INF_F ? 0.f : both, fade = exp2_fast(top - zero);
+      top = both;
+      sum *= fade;
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] *= fade;
+#pragma unroll
+      for (int k = 0; k < AT_ONCE; ++k) {
+        const float f = exp2_fast(m[k] - zero);
+        sum += l[k] * f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] += x[k][e] * f;
+      }
     }
-    float both = top;
+  };
+  auto place = [&](int row, int& t) -> T* {         // of a row's result
+    const int r = at_line % p.row_tiles * tile_rows + row, head = at_line / p.row_tiles * p.group + r % p.group;
+    t = r / p.group;
+    return static_cast<T*>(p.out) + (((long long)b * p.tokens + t) * p.heads + head) * p.D;
+  };
+  const int count = last - first + 1;
+  int t;
+  if (count <= AT_ONCE) {
+    for (int r = warp; r < rows; r += WARPS) {
+      gather(row0 + r, first, last + 1);
+      T* dst = place(row0 + r, t) + lane * E;
+      const float inv = inverse_sum(p, sum, b, t, length);
 #pragma unroll
-    for (int k = 0; k < AT_ONCE; ++k) both = fmaxf(both, m[k]);
-    const float zero = both == -CUDART_INF_F ? 0.f : both, fade = exp2_fast(top - zero);
-    top = both;
-    sum *= fade;
-#pragma unroll
-    for (int e = 0; e < E; ++e) v[e] *= fade;
-#pragma unroll
-    for (int k = 0; k < AT_ONCE; ++k) {
-      const float f = exp2_fast(m[k] - zero);
-      sum += l[k] * f;
-#pragma unroll
-      for (int e = 0; e < E; ++e) v[e] += x[k][e] * f;
+      for (int e = 0; e < E; e += 2)
+        if (lane * E + e < p.D) *reinterpret_cast<uint32_t*>(dst + e) = pack_pair<T>(v[e] * inv, v[e + 1] * inv);
     }
+    return;
   }
+  const int each = (count + WARPS - 1) / WARPS;
+  for (int r = 0; r < rows; ++r) {
+    gather(row0 + r, first + min(count, warp * each), first + min(count, (warp + 1) * each));
+    __syncthreads();
 #pragma unroll
-  for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = v[e];
-  if (lane == 0) {
-    sums[warp][DP] = top;
-    sums[warp][DP + 1] = sum;
-  }
-  __syncthreads();
-  float all = -CUDART_INF_F;
+    for (int e = 0; e < E; ++e) sums[warp][lane * E + e] = v[e];
+    if (lane == 0) {
+      sums[warp][DP] = top;
+      sums[warp][DP + 1] = sum;
+    }
+    __syncthreads();
+    float all = -CUDART_INF_F;
 #pragma unroll
-  for (int k = 0; k < WARPS; ++k) all = fmaxf(all, sums[k][DP]);
-  const float base = all == -CUDART_INF_F ? 0.f : all;
-  const int d = threadIdx.x;
-  float x = 0.f;
-  sum = 0.f;
+    for (int k = 0; k < WARPS; ++k) all = fmaxf(all, sums[k][DP]);
+    const float base = all == -CUDART_INF_F ? 0.f : all;
+    const int d = threadIdx.x;
+    float x = 0.f;
+    sum = 0.f;
 #pragma unroll
-  for (int k = 0; k < WARPS; ++k) {
-    const float f = exp2_fast(sums[k][DP] - base);
-    sum += sums[k][DP + 1] * f;
-    if (d < DP) x += sums[k][d] * f;
-  }
-  const int t = at_row / p.group, head = at_line / p.row_tiles * p.group + at_row % p.group;
-  if (d < p.D) {
-    const float y = x * inverse_sum(p, sum, b, t, length);
-    T* dst = static_cast<T*>(p.out) + (((long long)b * p.tokens + t) * p.heads + head) * p.D + d;
-    if constexpr (std::is_same_v<T, __half>) *dst = __float2half_rn(y); else *dst = __float2bfloat16_rn(y);
+    for (int k = 0; k < WARPS; ++k) {
+      const float f = exp2_fast(sums[k][DP] - base);
+      sum += sums[k][DP + 1] * f;
+      if (d < DP) x += sums[k][d] * f;
+    }
+    T* dst = place(row0 + r, t);
+    if (d < p.D) {
+      const float y = x * inverse_sum(p, sum, b, t, length);
+      if constexpr (std::is_same_v<T, __half>) dst[d] = __float2half_rn(y); else dst[d] = __float2bfloat16_rn(y);
+    }
   }
 }
 
@@ -745,8 +769,11 @@ int launch_attend(const AttendParams& p, cudaStream_t st) {
     if (dev < 64) configured[dev] = true;
   }
   I4TC_CUDA(launch_kernel(true, kernel, dim3((unsigned)(p.parts * p.lines)), kAttendThreads, S::kSmem, st, p));
-  const dim3 grid((unsigned)(p.batch * p.lines), (unsigned)(S::ROWS < p.rows ? S::ROWS : p.rows));
-  I4TC_CUDA(launch_kernel(true, attend_join_kernel<T, DP>, grid, kAttendThreads, 0, st, p, S::ROWS));
+  // A row a block where they are few, more where blocks would queue: 8192 blocks of a row took 14 us longer than 1024 of eight.
+  const int rows = S::ROWS < p.rows ? S::ROWS : p.rows, all = p.batch * p.lines * rows;
+  const int each = all > 4096 ? 8 : all > 1024 ? 4 : 1;
+  const dim3 grid((unsigned)(p.batch * p.lines), (unsigned)((rows + each - 1) / each));
+  I4TC_CUDA(launch_kernel(true, attend_join_kernel<T, DP>, grid, kJoinThreads, 0, st, p, S::ROWS, each));
   return I4TC_OK;
 }
 template <typename T, int DP>
@@ -805,7 +832,7 @@ extern "C" int i4tc_tree_attention(const i4tc_tree_attention_args* a, int device
   p.rows = (int)rows; p.row_tiles = (int)((rows + 16 * warps - 1) / (16 * warps));
   p.lines = p.kv_heads * p.row_tiles;
   const int64_t most_length = a->table_width * a->page_size;
-  I4TC_REQUIRE(most_length < (1ll << 31) - 2 * kTile && a->batch * ((most_length + a->tokens) / kTile + 1) < (1ll << 31) && a->batch * p.lines < (1ll << 31),
+  I4TC_REQUIRE(most_length < (1ll << 31) - 2 * kTile && a->batch * ((most_length + a->tokens) / kTile + 1) < (1ll << 31) && a->batch * p.lines < (1ll << 24),
                I4TC_EUNSUPPORTED, "the table has room for too many tokens");
   p.parts = attend_parts(info->sm_count, a->batch, p.lines, most_length, a->tokens);
   I4TC_REQUIRE(a->scratch_bytes >= (int64_t)p.parts * p.lines * 2 * (int64_t)slot_floats(16 * warps, padded_dim(p.D)) * 4, I4TC_EWORKSPACE,
