@@ -11,7 +11,8 @@ Mode selection follows the plugin's environment flags (``int4_native_tc/benchmar
   (one quantiser + one GEMM per layer, as ``int4_native_tc/profile_layer.py:83-119``);
 * ``INT4TC_CLIP_RATIO=r`` (0 < r <= 1, default 1): outlier clipping of the activation range;
 * ``INT4TC_CALIBRATION_STATS=file`` (+ ``INT4TC_SQ_ALPHA``, default 0.5): SmoothQuant factors from the
-  collector's statistics file, baked into the weight at load time and divided out of the activations.
+  collector's statistics file, baked into the weight at load time and divided out of the activations;
+* ``INT4TC_ACT_BITS=16``: activations stay in 16 bits (decoding: the weights are read once for every 32 tokens), in either scale mode.
 """
 from __future__ import annotations
 
@@ -49,7 +50,7 @@ class W4A4Int4TCLinearMethod:
 
     def __init__(self, per_channel: bool | None = None, asymmetric: bool | None = None,
                  clip_ratio: float | None = None, calibration_stats=None, sq_alpha: float | None = None,
-                 layer_name: str | None = None):
+                 layer_name: str | None = None, act_bits: int | None = None):
         env = os.environ
         self.per_channel = per_channel_from_env() if per_channel is None else per_channel
         self.asymmetric = (env.get("INT4TC_ASYMMETRIC", "0") == "1") if asymmetric is None else asymmetric
@@ -61,6 +62,11 @@ class W4A4Int4TCLinearMethod:
             calibration_stats = env.get("INT4TC_CALIBRATION_STATS") or None
         self.calibration_stats = calibration_stats
         self.layer_name = layer_name
+        self.act_bits = int(env.get("INT4TC_ACT_BITS", "4")) if act_bits is None else int(act_bits)
+        if self.act_bits not in (4, 16):
+            raise ValueError("activations have 4 or 16 bits")
+        if self.act_bits == 16 and (self.asymmetric or self.clip_ratio < 1.0):
+            raise ValueError("asymmetric codes and clipping belong to 4-bit activations")
         if self.per_channel and (self.asymmetric or self.clip_ratio < 1.0 or calibration_stats is not None):
             raise ValueError("asymmetric codes, clipping and SmoothQuant belong to the per-group configuration")
 
@@ -111,7 +117,10 @@ class W4A4Int4TCLinearMethod:
         N = layer.output_size_per_partition
         x2d = x.reshape(-1, K)
         M = x2d.shape[0]
-        if self.per_channel:
+        if self.act_bits == 16:
+            sm = getattr(layer, "smooth_scale", None)
+            out = ops.w4a16_linear(x2d if sm is None else x2d / sm.to(x2d.dtype), layer.weight_int4, layer.weight_scale, N, self.per_channel)
+        elif self.per_channel:
             out = ops.linear(x2d, layer.weight_int4, layer.weight_scale, N, True)
         elif self.asymmetric:
             sm = getattr(layer, "smooth_scale", None)

@@ -2,6 +2,9 @@
 (36 layers, hidden 4096, 32 query / 8 KV heads, head_dim 128, SwiGLU 12288,
 RMSNorm, RoPE; attention stays in bf16 through torch SDPA).  Random-initialised weights: this is a
 throughput harness for the caller side of the op boundary, not a checkpoint loader.
+
+Decoding: ``prefill`` fills a paged cache (``DecodeCache``), ``step`` takes one token, a chain or a tree of drafts of every sequence
+through the same packed weights with 16-bit activations, and ``commit`` keeps the accepted ones.
 """
 from __future__ import annotations
 
@@ -111,23 +114,47 @@ class Block(nn.Module):
             lin.weight.data[r0:r1] = (torch.randn(r1 - r0, k, device=device, generator=gen) * 0.02).to(torch.bfloat16)
         return lin.quantize_()  # the bf16 weight is released here
 
-    def forward(self, x, cos, sin):
+    def forward(self, x, cos, sin, attend=None):
         cfg = self.cfg
         B, S, _ = x.shape
         if self.fused:
-            return self._forward_fused(x, cos, sin)
+            return self._forward_fused(x, cos, sin, attend)
         qkv = self.qkv(self.ln1(x))
+        if attend is not None:
+            return self._feed_forward(x + self.o(attend(self, qkv)))
         q, k, v = qkv.split([cfg.q_heads * cfg.head_dim, cfg.kv_heads * cfg.head_dim, cfg.kv_heads * cfg.head_dim], -1)
         q = self.q_norm(q.view(B, S, cfg.q_heads, cfg.head_dim)).transpose(1, 2)
         k = self.k_norm(k.view(B, S, cfg.kv_heads, cfg.head_dim)).transpose(1, 2)
         v = v.view(B, S, cfg.kv_heads, cfg.head_dim).transpose(1, 2)
         q, k = apply_rope(q, cos, sin), apply_rope(k, cos, sin)
         a = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
-        x = x + self.o(a.transpose(1, 2).reshape(B, S, -1))
+        return self._feed_forward(x + self.o(a.transpose(1, 2).reshape(B, S, -1)))
+
+    def _feed_forward(self, x):
         gu = self.gate_up(self.ln2(x))
-        g, u = gu.split(cfg.inter, -1)
+        g, u = gu.split(self.cfg.inter, -1)
         return x + self.down(F.silu(g) * u)
 
+    def _turned_heads(self, qkv, positions, freqs):
+        """Query, key and value heads [tokens, heads, head_dim] of qkv [tokens, width], normed and at their positions."""
+        cfg = self.cfg
+        q, k, v = qkv.view(qkv.shape[0], -1, cfg.head_dim).split([cfg.q_heads, cfg.kv_heads, cfg.kv_heads], 1)
+        return ops.rope_(self.q_norm(q), positions, freqs), ops.rope_(self.k_norm(k), positions, freqs), v
+
+    def step(self, x, positions, freqs, attend):
+        """x [B, T, hidden] through the layer with 16-bit activations and ``attend(q, k, v)`` over [B, T, heads, head_dim]."""
+        cfg = self.cfg
+        B, T, H = x.shape
+
+        def linear(lin, y):
+            return ops.w4a16_linear(y, lin.weight_int4, lin.weight_scale, lin.out_features, lin.method.per_channel)
+
+        heads = self._turned_heads(linear(self.qkv, self.ln1(x).view(B * T, H)), positions, freqs)
+        a = attend(*(t.unflatten(0, (B, T)) for t in heads))
+        x = x + linear(self.o, a.view(B * T, -1)).view(B, T, H)
+        up = ops.w4a16_gated_linear(self.ln2(x).view(B * T, H), self.gate_up.weight_int4, self.gate_up.weight_scale, cfg.inter,
+                                    self.gate_up.method.per_channel)
+        return x + linear(self.down, up).view(B, T, H)
 
     def _attention(self, qkv, B, S, cos, sin):
         cfg = self.cfg
@@ -150,18 +177,46 @@ class Block(nn.Module):
         a = F.scaled_dot_product_attention(q, k, v, is_causal=True, enable_gqa=True)
         return a.transpose(1, 2).reshape(B, S, -1)
 
-    def _forward_fused(self, x, cos, sin):
+    def _forward_fused(self, x, cos, sin, attend=None):
         """Per-group mode with the quantisers folded into the ops in front of them: RMSNorm + quantise in one
         kernel before qkv and gate+up, SwiGLU + quantise in one kernel before down."""
         B, S, H = x.shape
         M = B * S
         xp, xs = ops.rmsnorm_int4_quant_grouped(x.view(M, H), self.ln1.weight, self.ln1.eps)
         qkv = apply_quantized(self.qkv, xp, xs, M).view(B, S, -1)
-        x = x + self.o(self._attention(qkv, B, S, cos, sin))
+        x = x + self.o(self._attention(qkv, B, S, cos, sin) if attend is None else attend(self, qkv))
         xp, xs = ops.rmsnorm_int4_quant_grouped(x.view(M, H), self.ln2.weight, self.ln2.eps)
         gu = apply_quantized(self.gate_up, xp, xs, M)
         ap, asc = _moe.moe_silu_mul_quant(gu)
         return x + apply_quantized(self.down, ap, asc, M).view(B, S, H)
+
+
+class DecodeCache:
+    """Paged keys and values of a batch: ``k`` and ``v`` hold [pages, page_size, kv_heads, head_dim] for each layer, a sequence's pages
+    are in ``block_table`` [batch, width] and its tokens counted in ``lengths`` [batch] (int32, on the device).  Here every sequence
+    owns its pages from the start; a server hands them out by writing the table."""
+
+    def __init__(self, cfg: Qwen3Config, batch: int, tokens: int, page_size: int = 64, device="cuda"):
+        width = -(-tokens // page_size)
+        shape = (batch * width, page_size, cfg.kv_heads, cfg.head_dim)
+        self.k, self.v = ([torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(cfg.layers)] for _ in range(2))
+        self.block_table = torch.arange(batch * width, dtype=torch.int32, device=device).view(batch, width)
+        self.lengths = torch.zeros(batch, dtype=torch.int32, device=device)
+        self.freqs = ops.rope_frequencies(cfg.head_dim, cfg.rope_theta, device)[0]
+        self.pending: list = []       # keys and values of the last step, layer by layer, not yet in the cache
+
+    def append(self, layer: int, k, v, counts=None, select=None) -> None:
+        ops.kv_cache_append_(self.k[layer], self.v[layer], k, v, self.block_table, self.lengths, select=select, counts=counts)
+
+    def commit(self, counts: torch.Tensor | None = None, select: torch.Tensor | None = None) -> None:
+        """Keeps ``counts[b]`` tokens of the last step (all without): its first ones, or rows ``select[b, :counts[b]]``, the accepted path of a
+        tree.  int32; nothing waits for the device."""
+        if not self.pending:
+            raise RuntimeError("commit: there is no step to keep tokens of")
+        for layer, (k, v) in enumerate(self.pending):
+            self.append(layer, k, v, counts, select)
+        self.lengths += self.pending[0][0].shape[1] if counts is None else counts
+        self.pending = []
 
 
 class Qwen3Prefill(nn.Module):
@@ -181,4 +236,46 @@ class Qwen3Prefill(nn.Module):
         cos, sin = rope_tables(ids.shape[1], self.cfg.head_dim, self.cfg.rope_theta, ids.device)
         for blk in self.blocks:
             x = blk(x, cos, sin)
+        return self.norm(x)
+
+    @torch.no_grad()
+    def prefill(self, ids: torch.Tensor, cache: DecodeCache, counts: torch.Tensor | None = None) -> torch.Tensor:
+        """As ``forward`` for prompts [B, S] of which ``counts[b]`` tokens count (int32; all without), whose keys and values go into the empty
+        sequences of ``cache``."""
+        cfg = self.cfg
+        B, S = ids.shape
+        freqs = cache.freqs
+        positions = torch.arange(S, device=ids.device).repeat(B)
+        x = self.embed(ids)
+        for layer, blk in enumerate(self.blocks):
+            def attend(blk, qkv, layer=layer):
+                q, k, v = (t.unflatten(0, (B, S)) for t in blk._turned_heads(qkv.reshape(B * S, -1), positions, freqs))
+                cache.append(layer, k, v, counts)
+                a = F.scaled_dot_product_attention(*(t.transpose(1, 2) for t in (q, k, v)), is_causal=True, enable_gqa=True)
+                return a.transpose(1, 2).reshape(B, S, -1)
+
+            x = blk(x, None, None, attend)
+        cache.lengths += S if counts is None else counts
+        return self.norm(x)
+
+    @torch.no_grad()
+    def step(self, ids: torch.Tensor, cache: DecodeCache, tree_mask: torch.Tensor | None = None) -> torch.Tensor:
+        """One token, a chain or a tree of drafts of every sequence: ids [B, T] -> final hidden states [B, T, hidden].  In a tree node t sees
+        the nodes j with ``tree_mask[b, t, j]`` (bool, itself and its ancestors) and stands that many positions behind the cache.
+        ``cache.commit`` keeps the accepted ones; until then the cache is as it was, and the next ``step`` forgets them."""
+        B, T = ids.shape
+        freqs = cache.freqs
+        if tree_mask is None:
+            depth = torch.arange(T, device=ids.device)
+        else:
+            depth = tree_mask.sum(-1) - 1
+        positions = (cache.lengths[:, None] + depth).flatten()
+        x = self.embed(ids)
+        cache.pending = []
+        for layer, blk in enumerate(self.blocks):
+            def attend(q, k, v, layer=layer):
+                cache.pending.append((k, v))
+                return ops.tree_attention(q, k, v, cache.k[layer], cache.v[layer], cache.block_table, cache.lengths, tree_mask=tree_mask)
+
+            x = blk.step(x, positions, freqs, attend)
         return self.norm(x)
