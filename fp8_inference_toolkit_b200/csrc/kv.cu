@@ -88,6 +88,11 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
 // as the result where it holds all of it, else as maximum, sum and weighted values (fp32) to scratch, and a second kernel adds a
 // sequence's parts in ascending order.  No atomics: the same bits in every run.
 //
+// Short sequences (by the room in their table) take another way, without scratch and in one kernel: a cluster of up to eight blocks
+// shares one (sequence, kv head, row tile), each takes an equal run of its tiles, and the blocks' sums are added in order through
+// distributed shared memory.  One token over 1001 takes the same 11 us on the device, and the host one
+// launch and one allocation less (14 us a call instead of 19).
+//
 // A block's four warps are WR row warps (16 rows each) times 4 / WR key warps, which share out a tile's keys and are added at the
 // item's end: few rows do not leave warps idle.  Tiles arrive by cp.async, two ahead; a key's address (its page) is looked
 // up one tile before that.
@@ -106,6 +111,7 @@ struct AttendParams {
   int rows, row_tiles;          // of an item: tokens * group
   int lines;                    // kv heads times row tiles: blocks of a part
   int parts;                    // of the line, at most
+  int ranks;                    // blocks of a cluster, where a sequence has its own; else 0
   float scale_log2;             // |scale| * log2(e), not zero: what is masked stays so
   uint32_t flip;                // sign bits of two queries, where the scale is negative
   unsigned int* status;
@@ -189,8 +195,9 @@ struct Cursor {
     length = line.length_of(p, b);
     tiles = tiles_of(p, length);
   }
+  template <bool OWN>
   __device__ __forceinline__ void next(const AttendParams& p, const Line& line) {
-    if (++tile < tiles) return;
+    if (++tile < tiles || OWN) return;
     tile = 0;
     ++b;
     open(p, line);
@@ -258,8 +265,8 @@ struct AttendShape {
   static constexpr int kSmem = kStages * 2 * kStage + kPlaces * kTile * 16 + kMerge;
 };
 
-// DP: D rounded up to 64 or 128 (the elements behind D are zeros in shared memory).
-template <typename T, int DP, int WR>
+// DP: D rounded up to 64 or 128 (the elements behind D are zeros in shared memory).  OWN: a cluster for each sequence and line.
+template <typename T, int DP, int WR, bool OWN>
 __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendParams p) {
   using S = AttendShape<DP, WR>;
   constexpr int CH = DP / 8;                        // 16-byte chunks of a row
@@ -279,17 +286,28 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
   pdl_wait();
   pdl_trigger();
 
-  const int part = blockIdx.x / p.lines, kvh = blockIdx.x % p.lines / p.row_tiles, tile_row0 = blockIdx.x % p.lines % p.row_tiles * S::ROWS;
+  const int block = OWN ? blockIdx.x / p.ranks : blockIdx.x, rank = OWN ? blockIdx.x % p.ranks : 0;
+  const int part = block / p.lines, kvh = block % p.lines / p.row_tiles, tile_row0 = block % p.lines % p.row_tiles * S::ROWS;
   Line line;
-  line.open(p, blockIdx.x == 0);
-  const int parts = min(p.parts, line.total);       // no part is empty
-  if (part >= parts) return;
-  const int first = part_start(line.total, parts, part), count = part_start(line.total, parts, part + 1) - first;
   Cursor cur;
-  int before;
-  cur.b = line.find(p, first, before);
-  cur.open(p, line);
-  cur.tile = first - before;
+  int count;
+  if constexpr (OWN) {
+    cur.b = part;
+    cur.length = cached(p, part, rank == 0);
+    cur.tiles = tiles_of(p, cur.length);
+    cur.tile = part_start(cur.tiles, p.ranks, rank);
+    count = part_start(cur.tiles, p.ranks, rank + 1) - cur.tile;
+  } else {
+    line.open(p, blockIdx.x == 0);
+    const int parts = min(p.parts, line.total);     // no part is empty
+    if (part >= parts) return;
+    const int first = part_start(line.total, parts, part);
+    count = part_start(line.total, parts, part + 1) - first;
+    int before;
+    cur.b = line.find(p, first, before);
+    cur.open(p, line);
+    cur.tile = first - before;
+  }
   Cursor ahead = cur;                               // whose places are looked up next
 
   // Places of the tile at `ahead`: key tid of it.  In two halves, the page's number and the addresses, so that nobody waits for the table.
@@ -340,7 +358,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
     pages[i] = 0;
     if (i < count) {
       if (tid < kTile) pages[i] = look_up(ahead);
-      ahead.next(p, line);
+      ahead.next<OWN>(p, line);
     }
   }
 #pragma unroll
@@ -586,7 +604,9 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
       }
       if (wk == 0) {
         const int row0 = tile_row0 + wr * 16 + g;
-        if (whole && ends) {
+        if (OWN && p.ranks > 1) {
+          // added below
+        } else if (OWN || (whole && ends)) {
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const int row = row0 + 8 * h;
@@ -618,13 +638,67 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
       }
       whole = true;
     }
-    const bool another = ends && i + 1 < count;
-    cur.next(p, line);
+    const bool another = !OWN && ends && i + 1 < count;
+    cur.next<OWN>(p, line);
     if (another) begin();
     if (more) {
       if (tid < kTile) places[((i + kStages) % kPlaces) * kTile + tid] = place_of(ahead, page);
-      ahead.next(p, line);
+      ahead.next<OWN>(p, line);
     }
+  }
+  if constexpr (OWN) {
+    if (p.ranks == 1) return;
+    // this block's sums where its tiles were, then every rank adds the rows rank, rank + ranks, ...
+    float* sums = reinterpret_cast<float*>(smem);   // values [rows][DP], then reference and sum [rows][2]
+    static_assert(S::ROWS * (DP + 2) * 4 <= kStages * 2 * S::kStage, "the sums fit the tiles' place");
+    __syncthreads();
+    if (wk == 0) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int row = wr * 16 + g + 8 * h;
+        float* dst = sums + row * DP + 2 * t4;
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<float2*>(dst + dt * 8) = make_float2(o[dt][2 * h], o[dt][2 * h + 1]);
+        if (t4 == 0) *reinterpret_cast<float2*>(sums + S::ROWS * DP + row * 2) = make_float2(m[h], l[2 * h]);
+      }
+    }
+    ptx::cluster_sync();
+    constexpr int E = DP / 32;
+    const uint32_t base = stage0;
+    for (int row = rank + p.ranks * warp; row < S::ROWS && tile_row0 + row < p.rows; row += p.ranks * (kAttendThreads / 32)) {
+      float top = -CUDART_INF_F, sum = 0.f, v[E];
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[e] = 0.f;
+      float ms[8], ls[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        ms[k] = -CUDART_INF_F;
+        ls[k] = 0.f;
+        if (k < p.ranks)
+          asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(ms[k]), "=f"(ls[k]) : "r"(ptx::mapa_shared(base + (S::ROWS * DP + row * 2) * 4, k)));
+        top = fmaxf(top, ms[k]);
+      }
+      const float zero = top == -CUDART_INF_F ? 0.f : top;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (k >= p.ranks) break;
+        const float f = exp2_fast(ms[k] - zero);
+        sum += ls[k] * f;
+        const uint32_t from = ptx::mapa_shared(base + (row * DP + lane * E) * 4, k);
+        float x[E];
+        if constexpr (E == 4) asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]) : "r"(from));
+        else asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x[0]), "=f"(x[1]) : "r"(from));
+#pragma unroll
+        for (int e = 0; e < E; ++e) v[e] += x[e] * f;
+      }
+      const int r = tile_row0 + row, t = r / p.group;
+      const float inv = inverse_sum(p, sum, part, t, cached(p, part, false));
+      T* dst = static_cast<T*>(p.out) + (((long long)part * p.tokens + t) * p.heads + kvh * p.group + r % p.group) * p.D + lane * E;
+#pragma unroll
+      for (int e = 0; e < E; e += 2)
+        if (lane * E + e < p.D) *reinterpret_cast<uint32_t*>(dst + e) = pack_pair<T>(v[e] * inv, v[e + 1] * inv);
+    }
+    ptx::cluster_sync();   // the others may still be reading
   }
 }
 
@@ -751,16 +825,31 @@ __global__ void __launch_bounds__(kJoinThreads) attend_join_kernel(const AttendP
 
 int row_warps(int64_t rows) { return rows <= 16 ? 1 : rows <= 32 ? 2 : 4; }
 int padded_dim(int64_t D) { return D <= 64 ? 64 : 128; }
-// Parts of the line: two blocks an SM in all.
-int attend_parts(int sm_count, int64_t batch, int64_t lines, int64_t most_length, int64_t tokens) {
-  const int64_t tiles = batch * ((most_length + tokens + kTile - 1) / kTile), most = (int64_t)sm_count * 2 / lines;
-  return (int)(most < 1 ? 1 : tiles < most ? tiles : most);
+// How the work is shared out: clusters of `ranks` blocks for each sequence and line, or (0) parts of the line, two blocks an SM in all.
+struct AttendPlan {
+  int ranks, parts;
+};
+AttendPlan attend_plan(int sm_count, int64_t batch, int64_t lines, int64_t most_length, int64_t tokens) {
+  const int64_t tiles = (most_length + tokens + kTile - 1) / kTile, slots = (int64_t)sm_count * 2;
+  const int64_t most = slots / lines < 1 ? 1 : slots / lines;
+  AttendPlan plan = {0, (int)(batch * tiles < most ? batch * tiles : most)};
+  // Microseconds, by the room in the table: a block's way to its first tile and its end, its tiles, and for parts the second kernel.
+  double best = 4.0 + 5.0 + 1.1 * (double)((batch * tiles + plan.parts - 1) / plan.parts) * ((plan.parts * lines + slots - 1) / slots);
+  for (int ranks = 1; ranks <= 8; ranks *= 2) {
+    const int64_t waves = (batch * lines * ranks + slots - 1) / slots;
+    const double cost = waves * (4.0 + 1.1 * (double)((tiles + ranks - 1) / ranks)) + (ranks > 1 ? 1.5 : 0.0);
+    if (cost < best && batch * lines * ranks < (1ll << 30)) {
+      best = cost;
+      plan.ranks = ranks;
+    }
+  }
+  return plan;
 }
 
-template <typename T, int DP, int WR>
+template <typename T, int DP, int WR, bool OWN>
 int launch_attend(const AttendParams& p, cudaStream_t st) {
   using S = AttendShape<DP, WR>;
-  auto kernel = attend_kernel<T, DP, WR>;
+  auto kernel = attend_kernel<T, DP, WR, OWN>;
   static bool configured[64] = {false};
   int dev = 0;
   I4TC_CUDA(cudaGetDevice(&dev));
@@ -768,17 +857,41 @@ int launch_attend(const AttendParams& p, cudaStream_t st) {
     I4TC_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
     if (dev < 64) configured[dev] = true;
   }
-  I4TC_CUDA(launch_kernel(true, kernel, dim3((unsigned)(p.parts * p.lines)), kAttendThreads, S::kSmem, st, p));
-  // A row a block where they are few, more where blocks would queue: 8192 blocks of a row took 14 us longer than 1024 of eight.
-  const int rows = S::ROWS < p.rows ? S::ROWS : p.rows, all = p.batch * p.lines * rows;
-  const int each = all > 4096 ? 8 : all > 1024 ? 4 : 1;
-  const dim3 grid((unsigned)(p.batch * p.lines), (unsigned)((rows + each - 1) / each));
-  I4TC_CUDA(launch_kernel(true, attend_join_kernel<T, DP>, grid, kJoinThreads, 0, st, p, S::ROWS, each));
+  if constexpr (OWN) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(p.batch * p.lines * p.ranks), 1, 1);
+    cfg.blockDim = dim3(kAttendThreads, 1, 1);
+    cfg.dynamicSmemBytes = S::kSmem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = (unsigned)p.ranks;
+    attr[1].val.clusterDim.y = 1;
+    attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = p.ranks > 1 ? 2 : 1;
+    I4TC_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+  } else {
+    I4TC_CUDA(launch_kernel(true, kernel, dim3((unsigned)(p.parts * p.lines)), kAttendThreads, S::kSmem, st, p));
+    // A row a block where they are few, more where blocks would queue: 8192 blocks of a row took 14 us longer than 1024 of eight.
+    const int rows = S::ROWS < p.rows ? S::ROWS : p.rows, all = p.batch * p.lines * rows;
+    const int each = all > 4096 ? 8 : all > 1024 ? 4 : 1;
+    const dim3 grid((unsigned)(p.batch * p.lines), (unsigned)((rows + each - 1) / each));
+    I4TC_CUDA(launch_kernel(true, attend_join_kernel<T, DP>, grid, kJoinThreads, 0, st, p, S::ROWS, each));
+  }
   return I4TC_OK;
 }
-template <typename T, int DP>
+
+template <typename T, int DP, bool OWN>
 int launch_rows(const AttendParams& p, int warps, cudaStream_t st) {
-  return warps == 1 ? launch_attend<T, DP, 1>(p, st) : warps == 2 ? launch_attend<T, DP, 2>(p, st) : launch_attend<T, DP, 4>(p, st);
+  return warps == 1 ? launch_attend<T, DP, 1, OWN>(p, st) : warps == 2 ? launch_attend<T, DP, 2, OWN>(p, st) : launch_attend<T, DP, 4, OWN>(p, st);
+}
+template <typename T>
+int launch_dim(const AttendParams& p, int warps, cudaStream_t st) {
+  if (padded_dim(p.D) == 64) return p.ranks ? launch_rows<T, 64, true>(p, warps, st) : launch_rows<T, 64, false>(p, warps, st);
+  return p.ranks ? launch_rows<T, 128, true>(p, warps, st) : launch_rows<T, 128, false>(p, warps, st);
 }
 
 }  // namespace
@@ -794,7 +907,8 @@ extern "C" int64_t i4tc_tree_attention_scratch_bytes(int64_t batch, int64_t toke
   const int64_t rows = tokens * (heads / kv_heads);
   const int tile_rows = 16 * row_warps(rows);
   const int64_t lines = kv_heads * ((rows + tile_rows - 1) / tile_rows);
-  return attend_parts(info->sm_count, batch, lines, most_length, tokens) * lines * 2 * (int64_t)slot_floats(tile_rows, padded_dim(D)) * 4;
+  const AttendPlan plan = attend_plan(info->sm_count, batch, lines, most_length, tokens);
+  return plan.ranks ? 0 : plan.parts * lines * 2 * (int64_t)slot_floats(tile_rows, padded_dim(D)) * 4;
 }
 
 extern "C" int i4tc_tree_attention(const i4tc_tree_attention_args* a, int device, void* stream) {
@@ -808,7 +922,7 @@ extern "C" int i4tc_tree_attention(const i4tc_tree_attention_args* a, int device
   I4TC_REQUIRE(a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->heads <= 65536, I4TC_EINVAL, "heads must be a multiple of kv_heads");
   I4TC_REQUIRE(a->batch <= 65536 && a->pages >= 0 && a->pages < (1ll << 31) && a->page_size > 0 && a->page_size < (1ll << 31) &&
                    a->table_width >= 0 && a->table_width < (1ll << 31), I4TC_EINVAL, "bad size");
-  I4TC_REQUIRE(a->q && a->k && a->v && a->lengths && a->out && a->scratch, I4TC_EINVAL, "null pointer");
+  I4TC_REQUIRE(a->q && a->k && a->v && a->lengths && a->out, I4TC_EINVAL, "null pointer");
   I4TC_REQUIRE(a->table_width == 0 || a->pages == 0 || (a->k_cache && a->v_cache && a->block_table), I4TC_EINVAL, "null pointer");
   I4TC_REQUIRE(aligned_to(a->k, 16) && aligned_to(a->v, 16) && aligned_to(a->k_cache, 16) && aligned_to(a->v_cache, 16) &&
                    aligned_to(a->q, 4) && aligned_to(a->out, 16) && aligned_to(a->scratch, 16) && a->q_batch % 2 == 0 && a->q_token % 2 == 0 &&
@@ -834,8 +948,11 @@ extern "C" int i4tc_tree_attention(const i4tc_tree_attention_args* a, int device
   const int64_t most_length = a->table_width * a->page_size;
   I4TC_REQUIRE(most_length < (1ll << 31) - 2 * kTile && a->batch * ((most_length + a->tokens) / kTile + 1) < (1ll << 31) && a->batch * p.lines < (1ll << 24),
                I4TC_EUNSUPPORTED, "the table has room for too many tokens");
-  p.parts = attend_parts(info->sm_count, a->batch, p.lines, most_length, a->tokens);
-  I4TC_REQUIRE(a->scratch_bytes >= (int64_t)p.parts * p.lines * 2 * (int64_t)slot_floats(16 * warps, padded_dim(p.D)) * 4, I4TC_EWORKSPACE,
+  const AttendPlan plan = attend_plan(info->sm_count, a->batch, p.lines, most_length, a->tokens);
+  p.parts = plan.parts;
+  p.ranks = plan.ranks;
+  I4TC_REQUIRE(p.ranks || a->scratch != nullptr, I4TC_EINVAL, "null pointer");
+  I4TC_REQUIRE(p.ranks || a->scratch_bytes >= (int64_t)p.parts * p.lines * 2 * (int64_t)slot_floats(16 * warps, padded_dim(p.D)) * 4, I4TC_EWORKSPACE,
                "the scratch is too small");
   p.scale_log2 = fmaxf((float)(fabs(a->scale) * 1.4426950408889634), 1e-30f);
   p.flip = a->scale < 0 ? 0x80008000u : 0u;
@@ -843,11 +960,7 @@ extern "C" int i4tc_tree_attention(const i4tc_tree_attention_args* a, int device
   DeviceGuard guard(device);
   I4TC_CUDA(guard.err);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  auto pick = [&](auto type) {
-    using T = decltype(type);
-    return padded_dim(p.D) == 64 ? launch_rows<T, 64>(p, warps, st) : launch_rows<T, 128>(p, warps, st);
-  };
-  return a->dtype == I4TC_BF16 ? pick(__nv_bfloat16{}) : pick(__half{});
+  return a->dtype == I4TC_BF16 ? launch_dim<__nv_bfloat16>(p, warps, st) : launch_dim<__half>(p, warps, st);
 }
 
 extern "C" int i4tc_kv_append(const i4tc_kv_append_args* a, int device, void* stream) {

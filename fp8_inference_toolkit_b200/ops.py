@@ -808,9 +808,9 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     pages, page = k_cache.shape[:2]
     width = block_table.shape[1]
     nbytes = lib.i4tc_tree_attention_scratch_bytes(B, T, H, Hk, D, width * page, index)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
     args = _ATTENTION_ARGS.pack(q_at, k_at, v_at, k_cache_at, v_cache_at, block_table.data_ptr(), lengths.data_ptr(), mask_at, out.data_ptr(),
-                                scratch.data_ptr(), nbytes, code, B, T, H, Hk, D, pages, page, width, sq[0], sq[1], sq[2], new[0], new[1], new[2],
+                                0 if scratch is None else scratch.data_ptr(), nbytes, code, B, T, H, Hk, D, pages, page, width, sq[0], sq[1], sq[2], new[0], new[1], new[2],
                                 cache[0], cache[1], cache[2], block_table.stride(0), mask_batch, D ** -0.5 if scale is None else scale)
     rc = lib.i4tc_tree_attention(args, index, _raw_stream(index) if _raw_stream is not None else _stream(q))
     if rc:

@@ -434,8 +434,8 @@ int i4tc_rope(const void* x, int dtype, int64_t tokens, int64_t heads, int64_t D
  * apart, 0 for one that all share; NULL: j <= t).  A token that sees nothing gives zeros.  Strides in elements, multiples of 8
  * (queries: of 2); k and v share theirs, the caches share theirs.  At most 64 new tokens, D a multiple of 8 up to 128.  Lengths
  * beyond the table and pages out of range set bit 2 of the status word (i4tc_check_status), and read nothing.
- * scratch: i4tc_tree_attention_scratch_bytes with most_length = table_width * page_size; free again when the call's
- * work on its stream is done. */
+ * scratch: i4tc_tree_attention_scratch_bytes with most_length = table_width * page_size (0 for short tables: NULL will do); free
+ * again when the call's work on its stream is done. */
 typedef struct {
   const void *q, *k, *v, *k_cache, *v_cache;
   const int32_t *block_table, *lengths;

@@ -89,15 +89,26 @@ CASES = [
 ]
 
 
+def _roomy(table, page):
+    """The table with room for 64 thousand tokens, what is not used of it not a page: the work is shared out in another way."""
+    wide = torch.full((table.shape[0], -(-65536 // page)), -1, dtype=torch.int32, device="cuda")
+    wide[:, :table.shape[1]] = table
+    return wide
+
+
+@pytest.mark.parametrize("room", [False, True])
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("B,T,H,Hk,D,page,lengths,tree", CASES)
-def test_attention(B, T, H, Hk, D, page, lengths, tree, dtype):
+def test_attention(B, T, H, Hk, D, page, lengths, tree, dtype, room):
+    """With a table that just holds the sequences, and with one that has room for many more tokens."""
     from fp8_inference_toolkit_b200 import ops
 
     gen = torch.Generator(device="cuda").manual_seed(B * 1000 + T)
     width = max(1, -(-max(lengths) // page)) + 1
     kc, vc, table = _pages(gen, B, page, width, Hk, D, dtype)
     q, k, v = _new(gen, B, T, H, Hk, D, dtype)
+    if room:
+        table = _roomy(table, page)
     n = torch.tensor(lengths, dtype=torch.int32, device="cuda")
     mask = _tree(torch.Generator().manual_seed(T), B, T) if tree else None
     out = ops.tree_attention(q, k, v, kc, vc, table, n, tree_mask=mask)
@@ -108,22 +119,25 @@ def test_attention(B, T, H, Hk, D, page, lengths, tree, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("room", [False, True])
 @pytest.mark.parametrize("T,H", [(1, 4), (6, 4), (20, 4), (40, 8)])
-def test_large_scores_and_scales(T, H, dtype):
+def test_large_scores_and_scales(T, H, dtype, room):
     """Scores of hundreds: the running maximum moves by more than an exponential holds; also a negative scale and a scale of zero."""
     from fp8_inference_toolkit_b200 import ops
 
     gen = torch.Generator(device="cuda").manual_seed(T)
     kc, vc, table = _pages(gen, 2, 16, 20, 2, 64, dtype)
     q, k, v = _new(gen, 2, T, H, 2, 64, dtype)
+    table = _roomy(table, 16) if room else table
     n = torch.tensor([313, 100], dtype=torch.int32, device="cuda")
     mask = _tree(torch.Generator().manual_seed(3), 2, T)
     for scale in (4.0, -0.5, 0.0):
         _check(ops.tree_attention(q, k, v, kc, vc, table, n, mask, scale), *_reference(q, k, v, kc, vc, table, n, mask, scale))
 
 
+@pytest.mark.parametrize("room", [False, True])
 @pytest.mark.parametrize("T,H", [(4, 2), (12, 2), (40, 2)])
-def test_rows_that_see_nothing(T, H):
+def test_rows_that_see_nothing(T, H, room):
     """An empty row of the mask: zeros without a cache, the cache alone with one."""
     from fp8_inference_toolkit_b200 import ops
 
@@ -133,6 +147,7 @@ def test_rows_that_see_nothing(T, H):
     mask = _tree(torch.Generator().manual_seed(1), 3, T)
     mask[:, T // 2] = False
     mask[1] = False
+    table = _roomy(table, 16) if room else table
     n = torch.tensor([0, 0, 70], dtype=torch.int32, device="cuda")
     out = ops.tree_attention(q, k, v, kc, vc, table, n, mask)
     assert not out[1].any() and not out[0, T // 2].any() and out[2, T // 2].any()
@@ -140,8 +155,9 @@ def test_rows_that_see_nothing(T, H):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("room", [False, True])
 @pytest.mark.parametrize("T,H", [(5, 2), (13, 2), (60, 1), (30, 8)])
-def test_what_is_not_seen_has_no_part(T, H, dtype):
+def test_what_is_not_seen_has_no_part(T, H, dtype, room):
     """NaN and infinities in unused slots, foreign pages and unseen nodes change nothing; in a seen node they reach the rows that see it,
     and those only."""
     from fp8_inference_toolkit_b200 import ops
@@ -152,6 +168,7 @@ def test_what_is_not_seen_has_no_part(T, H, dtype):
     n = torch.tensor([77, 0], dtype=torch.int32, device="cuda")
     mask = _tree(torch.Generator().manual_seed(2), 2, T)
     mask[:, :, T - 1] = False                      # nobody sees the last node, itself included
+    table = _roomy(table, 16) if room else table
     clean = ops.tree_attention(q, k, v, kc, vc, table, n, mask)
     used = torch.zeros(kc.shape[:2], dtype=torch.bool, device="cuda")
     at = torch.arange(77, device="cuda")
@@ -213,14 +230,16 @@ def test_offsets_past_32_bits():
     ops.check_status()
 
 
+@pytest.mark.parametrize("room", [False, True])
 @pytest.mark.parametrize("bad", ["page", "negative page", "length", "negative length"])
-def test_out_of_range_is_reported(bad):
+def test_out_of_range_is_reported(bad, room):
     """Nothing outside the cache is read, the call before and after stay right, and check_status raises once."""
     from fp8_inference_toolkit_b200 import ops
 
     gen = torch.Generator(device="cuda").manual_seed(10)
     kc, vc, table = _pages(gen, 2, 16, 6, 2, 64, torch.bfloat16)
     q, k, v = _new(gen, 2, 3, 4, 2, 64, torch.bfloat16)
+    table = _roomy(table, 16) if room else table
     n = torch.tensor([90, 40], dtype=torch.int32, device="cuda")
     want = ops.tree_attention(q, k, v, kc, vc, table, n)
     ops.check_status()
@@ -228,7 +247,7 @@ def test_out_of_range_is_reported(bad):
     if "page" in bad:
         t2[0, 2] = kc.shape[0] if bad == "page" else -1
     else:
-        n2[0] = 6 * 16 + 1 if bad == "length" else -5
+        n2[0] = table.shape[1] * 16 + 1 if bad == "length" else -5
     out = ops.tree_attention(q, k, v, kc, vc, t2, n2)
     assert torch.equal(out[1], want[1])
     with pytest.raises(RuntimeError, match="out of range"):
