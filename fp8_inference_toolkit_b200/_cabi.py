@@ -77,8 +77,8 @@ SIGNATURES = {
     "i4tc_qk_norm_rope": (_i, [_p, _l, _l, _l, _l, _l, _p, _p, _p, _p, _f, _i, _p]),
     "i4tc_rmsnorm_quant_grouped": (_i, [_p, _l, _l, _l, _p, _f, _l, _p, _p, _i, _p]),
     "i4tc_moe_combine": (_i, [_p, _p, _p, _l, _l, _l, _p, _i, _p]),
-    "i4tc_w4a16_linear": (_i, [_p, _i, _l, _l, _l, _p, _p, _i, _i, _p, _l, _i, _p]),
-    "i4tc_rope": (_i, [_p, _i, _l, _l, _l, _l, _l, _l, _p, _i, _p, _i, _f, _i, _p, _l, _l, _i, _p]),
+    "i4tc_w4a16_linear": (_i, [C.c_char_p, _i, _p]),
+    "i4tc_rope": (_i, [C.c_char_p, _i, _p]),
     "i4tc_tree_attention_scratch_bytes": (_l, [_l, _l, _l, _l, _l, _l, _i]),
     "i4tc_tree_attention": (_i, [C.c_char_p, _i, _p]),
     "i4tc_kv_append": (_i, [C.c_char_p, _i, _p]),

@@ -16,8 +16,9 @@ constexpr unsigned kStatusRange = 4u;   // status word: a block table entry, a l
 
 // ---- append ------------------------------------------------------------------------------------------------------------
 // Row i < counts[b] of sequence b, taken from new row select[b, i] (i without select), goes to token lengths[b] + i.  Bound: the rows
-// read and written once.  A block takes a few rows; their places are looked up once, by a thread each.
-constexpr int kAppendThreads = 256;
+// read and written once.  A block takes a few rows; their places are looked up once, by a thread each.  A prompt of 8000 tokens of 8
+// heads of 128: 13.7 us with four accesses of a thread on their way together, 15.5 one by one.
+constexpr int kAppendThreads = 256, kAppendAtOnce = 4;   // AtOnce: a thread's accesses on their way together
 
 struct AppendParams {
   const void *k, *v;
@@ -62,14 +63,26 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(const AppendPara
   }
   __syncthreads();
   const int per_row = 2 * p.heads * p.row_units;   // keys, then values
-  for (int i = threadIdx.x; i < n * per_row; i += kAppendThreads) {
-    const int r = i / per_row, j = i - r * per_row;
-    if (to[r] < 0) continue;
-    const bool value = j >= per_row / 2;
-    const int c = value ? j - per_row / 2 : j, head = c / p.row_units, unit = c - head * p.row_units;
-    const char* src = static_cast<const char*>(value ? p.v : p.k) + from[r] + head * p.new_head;
-    char* dst = static_cast<char*>(value ? p.v_cache : p.k_cache) + to[r] + head * p.head_stride;
-    reinterpret_cast<V*>(dst)[unit] = reinterpret_cast<const V*>(src)[unit];
+  for (int i0 = threadIdx.x; i0 < n * per_row; i0 += kAppendThreads * kAppendAtOnce) {
+    V held[kAppendAtOnce];
+    char* dst[kAppendAtOnce];
+#pragma unroll
+    for (int k = 0; k < kAppendAtOnce; ++k) {
+      const int i = i0 + k * kAppendThreads;
+      dst[k] = nullptr;
+      if (i < n * per_row) {
+        const int r = i / per_row, j = i - r * per_row;
+        const bool value = j >= per_row / 2;
+        const int c = value ? j - per_row / 2 : j, head = c / p.row_units, unit = c - head * p.row_units;
+        if (to[r] >= 0) {
+          held[k] = reinterpret_cast<const V*>(static_cast<const char*>(value ? p.v : p.k) + from[r] + head * p.new_head)[unit];
+          dst[k] = static_cast<char*>(value ? p.v_cache : p.k_cache) + to[r] + head * p.head_stride + unit * sizeof(V);
+        }
+      }
+    }
+#pragma unroll
+    for (int k = 0; k < kAppendAtOnce; ++k)
+      if (dst[k] != nullptr) *reinterpret_cast<V*>(dst[k]) = held[k];
   }
 }
 
@@ -992,7 +1005,7 @@ extern "C" int i4tc_kv_append(const i4tc_kv_append_args* a, int device, void* st
                "operands must be aligned to their element size");
   p.row_units = (int)(a->head_dim * 2 / bytes);
   const long long rows = (long long)p.batch * p.tokens, per_row = 2ll * p.heads * p.row_units;
-  p.rows_each = (int)(4 * kAppendThreads / per_row);
+  p.rows_each = (int)(kAppendAtOnce * kAppendThreads / per_row);
   p.rows_each = p.rows_each < 1 || rows <= 2 * info->sm_count ? 1 : p.rows_each > kAppendThreads ? kAppendThreads : p.rows_each;
   const long long blocks = (rows + p.rows_each - 1) / p.rows_each;
   I4TC_REQUIRE(blocks < (1ll << 31) && per_row * p.rows_each < (1ll << 31), I4TC_EINVAL, "bad size");

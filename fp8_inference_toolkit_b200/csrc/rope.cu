@@ -119,9 +119,14 @@ __global__ void __launch_bounds__(kRopeThreads) rope_kernel(const RopeParams p) 
 
 using namespace i4tc;
 
-extern "C" int i4tc_rope(const void* x, int dtype, int64_t tokens, int64_t heads, int64_t D, int64_t R, int64_t x_token, int64_t x_head,
-                         const void* positions, int long_positions, const double* freqs, int interleaved, float scale, int inverse,
-                         void* out, int64_t out_token, int64_t out_head, int device, void* stream) {
+extern "C" int i4tc_rope(const i4tc_rope_args* a, int device, void* stream) {
+  I4TC_REQUIRE(a != nullptr, I4TC_EINVAL, "null pointer");
+  const void *x = a->x, *positions = a->positions;
+  void* out = a->out;
+  const int64_t dtype = a->dtype, tokens = a->tokens, heads = a->heads, D = a->D, R = a->R, x_token = a->x_token, x_head = a->x_head,
+                out_token = a->out_token, out_head = a->out_head;
+  const double* freqs = a->freqs;
+  const bool long_positions = a->long_positions != 0, interleaved = a->interleaved != 0;
   I4TC_REQUIRE(dtype == I4TC_BF16 || dtype == I4TC_FP16, I4TC_EUNSUPPORTED, "x must be bfloat16 or float16");
   I4TC_REQUIRE(tokens >= 0 && heads >= 0 && D >= 0 && R >= 0 && R % 2 == 0 && R <= D, I4TC_EINVAL,
                "the rotated part must be an even number of elements of a head");
@@ -138,7 +143,7 @@ extern "C" int i4tc_rope(const void* x, int dtype, int64_t tokens, int64_t heads
   RopeParams p = {};
   p.x = x; p.out = out; p.x_token = x_token; p.x_head = x_head; p.out_token = out_token; p.out_head = out_head;
   p.positions = positions; p.freqs = freqs; p.tokens = (int)tokens; p.heads = (int)heads; p.D = (int)D; p.R = (int)R;
-  p.scale = scale; p.long_positions = long_positions != 0; p.inverse = inverse != 0; p.in_place = in_place;
+  p.scale = (float)a->scale; p.long_positions = long_positions; p.inverse = a->inverse != 0; p.in_place = in_place;
   // the widest access that strides, parts and addresses are multiples of
   int vec = 8;
   const int64_t all = (interleaved ? R : R / 2) | (in_place ? 0 : D - R) | x_token | x_head | out_token | out_head;

@@ -479,8 +479,14 @@ int launch_tokens(const W4A16Params& p, dim3 grid, size_t smem, cudaStream_t st)
 
 using namespace i4tc;
 
-extern "C" int i4tc_w4a16_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* w, const float* w_scale,
-                                 int per_channel, int gated, void* out, int64_t N, int device, void* stream) {
+extern "C" int i4tc_w4a16_linear(const i4tc_w4a16_args* a, int device, void* stream) {
+  I4TC_REQUIRE(a != nullptr, I4TC_EINVAL, "null pointer");
+  const int64_t dtype = a->dtype, M = a->M, K = a->K, N = a->N, ldx = a->ldx;
+  const void* x = a->x;
+  const uint8_t* w = a->w;
+  const float* w_scale = a->w_scale;
+  void* out = a->out;
+  const bool per_channel = a->per_channel != 0, gated = a->gated != 0;
   I4TC_REQUIRE(dtype == I4TC_BF16 || dtype == I4TC_FP16, I4TC_EUNSUPPORTED, "activations must be bfloat16 or float16");
   I4TC_REQUIRE(M >= 0 && N >= 0 && K > 0, I4TC_EINVAL, "bad size");
   if (M == 0 || N == 0) return I4TC_OK;

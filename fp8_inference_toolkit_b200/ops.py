@@ -529,6 +529,12 @@ def _half_input(t: torch.Tensor, name: str, dim: int) -> None:
     _require(not (t.requires_grad and torch.is_grad_enabled()), f"{name} requires grad: the op has no backward pass, call it under torch.no_grad()")
 
 
+# Arguments of an entry point that takes a struct: one conversion for all of them.
+_W4A16_ARGS = struct.Struct("@4P7q").pack
+_ROPE_ARGS = struct.Struct("@4P12qd").pack
+_ATTENTION_ARGS = struct.Struct("@10P21qd").pack
+_APPEND_ARGS = struct.Struct("@8P16q").pack
+
 _HALF = {torch.bfloat16: _cabi.BF16, torch.float16: _cabi.FP16}
 # The ops below are called once or more a layer for a single token, where a microsecond of checks is a tenth of the call: what a good call
 # looks like is one expression, and the checks that name what is wrong run for the others.
@@ -569,8 +575,8 @@ def _w4a16(x: torch.Tensor, w_packed: torch.Tensor, w_scale: torch.Tensor, N: in
         x, ldx = x.clone(memory_format=torch.contiguous_format), K
         at = x.data_ptr()
     out = x.new_empty((M, N))
-    rc = lib.i4tc_w4a16_linear(at, code, M, K, ldx, w_packed.data_ptr(), w_scale.data_ptr(), per_channel, gated, out.data_ptr(), N, index,
-                               _raw_stream(index) if _raw_stream is not None else _stream(x))
+    args = _W4A16_ARGS(at, w_packed.data_ptr(), w_scale.data_ptr(), out.data_ptr(), code, M, K, ldx, N, per_channel, gated)
+    rc = lib.i4tc_w4a16_linear(args, index, _raw_stream(index) if _raw_stream is not None else _stream(x))
     if rc:
         check(rc, who)
     return out
@@ -657,8 +663,9 @@ def _rope(x, positions, freqs, interleaved, scale, inverse, in_place, who):
         st = ot = heads * D
     if heads == 1:
         sh = oh = D
-    rc = lib.i4tc_rope(x.data_ptr(), code, tokens, heads, D, R, st, sh, positions.data_ptr(), kind is torch.int64, freqs.data_ptr(), interleaved,
-                       scale, inverse, out.data_ptr(), ot, oh, index, _raw_stream(index) if _raw_stream is not None else _stream(x))
+    args = _ROPE_ARGS(x.data_ptr(), positions.data_ptr(), freqs.data_ptr(), out.data_ptr(), code, tokens, heads, D, R, st, sh, ot, oh,
+                      kind is torch.int64, interleaved, inverse, scale)
+    rc = lib.i4tc_rope(args, index, _raw_stream(index) if _raw_stream is not None else _stream(x))
     if rc:
         check(rc, who)
     return out
@@ -680,10 +687,6 @@ def rope_(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, interle
     return _rope(x, positions, freqs, interleaved, scale, inverse, True, "rope_")
 
 
-_ATTENTION_ARGS = struct.Struct("@10P21qd")
-_APPEND_ARGS = struct.Struct("@8P16q")
-
-
 def _check_cache(k_cache, v_cache, block_table, lengths, k, v) -> None:
     for t, name in ((k, "k"), (v, "v"), (k_cache, "k_cache"), (v_cache, "v_cache")):
         _half_input(t, name, 4)
@@ -703,16 +706,18 @@ def _check_cache(k_cache, v_cache, block_table, lengths, k, v) -> None:
 
 
 def _cache_pair(k_cache, v_cache, block_table, lengths, k, v):
-    """Checks of a paged cache and the new rows beside it; (k, v, their strides, cache strides, block_table, lengths), k and v with the same strides."""
+    """Checks of a paged cache and the new rows beside it: (k, v, their strides, the cache's strides, block_table, lengths, device index, the sizes
+    B, T, kv_heads, D, pages, page size, width of the table), k and v with the same strides."""
     kind, index = k.dtype, k.get_device()
     if not (kind in _HALF and index >= 0 and k.dim() == 4 and k_cache.dim() == 4 and block_table.dim() == 2 and lengths.dim() == 1):
         _check_cache(k_cache, v_cache, block_table, lengths, k, v)
-    B, _, H, D = shape = k.shape
-    _, page, cache_heads, cache_D = cache_shape = k_cache.shape
+    B, T, H, D = shape = k.shape
+    pages, page, cache_heads, cache_D = cache_shape = k_cache.shape
+    rows, width = block_table.shape
     new, cache = k.stride(), k_cache.stride()
     if not (v.dtype is kind and k_cache.dtype is kind and v_cache.dtype is kind and v.shape == shape and v_cache.shape == cache_shape
             and v_cache.stride() == cache and H == cache_heads and D == cache_D and page > 0 and (cache[3] == 1 or D <= 1)
-            and block_table.dtype is torch.int32 and lengths.dtype is torch.int32 and block_table.shape[0] == B and lengths.shape[0] == B
+            and block_table.dtype is torch.int32 and lengths.dtype is torch.int32 and rows == B and lengths.shape[0] == B
             and v.get_device() == index and k_cache.get_device() == index and v_cache.get_device() == index
             and block_table.get_device() == index and lengths.get_device() == index
             and not ((k.requires_grad or v.requires_grad or k_cache.requires_grad or v_cache.requires_grad) and torch.is_grad_enabled())):
@@ -722,9 +727,11 @@ def _cache_pair(k_cache, v_cache, block_table, lengths, k, v):
         new = k.stride()
         if v.stride() != new:   # axes of one element: any stride counts as contiguous
             v = v.as_strided(shape, new)
-    if block_table.stride(1) != 1 and block_table.shape[1] > 1:
+    if block_table.stride(1) != 1 and width > 1:
         block_table = block_table.contiguous()
-    return k, v, new, cache, block_table, lengths if lengths.is_contiguous() else lengths.contiguous()
+    if not lengths.is_contiguous():
+        lengths = lengths.contiguous()
+    return k, v, new, cache, block_table, lengths, index, (B, T, H, D, pages, page, width)
 
 
 def kv_cache_append_(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tensor, v: torch.Tensor, block_table: torch.Tensor,
@@ -734,13 +741,13 @@ def kv_cache_append_(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tens
     ``block_table[b, token // page_size]``, and comes from new row ``select[b, i]`` (``i`` without ``select``): a prompt, or the accepted path
     of a tree of drafts.  All index tensors int32.  ``lengths`` stay as they are.  Counts, rows, tokens and pages out of range
     write nothing and are raised by ``check_status``."""
-    k, v, new, cache, block_table, lengths = _cache_pair(k_cache, v_cache, block_table, lengths, k, v)
-    B, T, H, D = k.shape
-    index = k.get_device()
+    k, v, new, cache, block_table, lengths, index, sizes = _cache_pair(k_cache, v_cache, block_table, lengths, k, v)
+    B, T = sizes[:2]
     counts_at = select_at = select_stride = 0
     if counts is not None:
         _require(counts.dtype is torch.int32 and counts.dim() == 1 and counts.shape[0] == B and counts.get_device() == index, "counts must be int32 [batch]")
-        counts = counts.contiguous()
+        if not counts.is_contiguous():
+            counts = counts.contiguous()
         counts_at = counts.data_ptr()
     if select is not None:
         _require(select.dtype is torch.int32 and select.dim() == 2 and select.shape[0] == B and select.get_device() == index,
@@ -749,10 +756,8 @@ def kv_cache_append_(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tens
         if select.stride(1) != 1:
             select = select.contiguous()
         select_at, select_stride = select.data_ptr(), select.stride(0)
-    pages, page = k_cache.shape[:2]
-    args = _APPEND_ARGS.pack(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
-                             counts_at, select_at, 2, B, T, H, D, pages, page, block_table.shape[1], new[0], new[1], new[2], cache[0], cache[1],
-                             cache[2], block_table.stride(0), select_stride)
+    args = _APPEND_ARGS(k.data_ptr(), v.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), lengths.data_ptr(),
+                        counts_at, select_at, 2, *sizes, new[0], new[1], new[2], cache[0], cache[1], cache[2], block_table.stride(0), select_stride)
     rc = lib.i4tc_kv_append(args, index, _raw_stream(index) if _raw_stream is not None else _stream(k))
     if rc:
         check(rc, "kv_cache_append_")
@@ -774,11 +779,9 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     code = _HALF.get(kind)
     if code is None or q.dim() != 4 or q.get_device() < 0 or (q.requires_grad and torch.is_grad_enabled()):
         _half_input(q, "q", 4)
-    k, v, new, cache, block_table, lengths = _cache_pair(k_cache, v_cache, block_table, lengths, k, v)
+    k, v, new, cache, block_table, lengths, index, (Bk, Tk, Hk, Dk, pages, page, width) = _cache_pair(k_cache, v_cache, block_table, lengths, k, v)
     B, T, H, D = q.shape
-    Bk, Tk, Hk, Dk = k.shape
-    index = q.get_device()
-    if not (k.dtype is kind and k.get_device() == index and Bk == B and Tk == T and Dk == D and T <= 64 and D % 8 == 0 and 0 < D <= 128
+    if not (k.dtype is kind and q.get_device() == index and Bk == B and Tk == T and Dk == D and T <= 64 and D % 8 == 0 and 0 < D <= 128
             and Hk > 0 and H % Hk == 0):
         _require(kind == k.dtype and q.device == k.device, "queries must have the keys' dtype and device")
         _require(k.shape == (B, T, Hk, D), "q must be [B, T, heads, D] and k [B, T, kv_heads, D]")
@@ -805,11 +808,9 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
         k, v = (t.clone(memory_format=torch.contiguous_format) for t in (k, v))
         new, k_at, v_at = k.stride(), k.data_ptr(), v.data_ptr()
     _require((k_cache_at | v_cache_at) % 16 == 0 and (cache[0] | cache[1] | cache[2]) % 8 == 0, "cached heads must be 16-byte aligned")
-    pages, page = k_cache.shape[:2]
-    width = block_table.shape[1]
     nbytes = lib.i4tc_tree_attention_scratch_bytes(B, T, H, Hk, D, width * page, index)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=q.device) if nbytes else None
-    args = _ATTENTION_ARGS.pack(q_at, k_at, v_at, k_cache_at, v_cache_at, block_table.data_ptr(), lengths.data_ptr(), mask_at, out.data_ptr(),
+    args = _ATTENTION_ARGS(q_at, k_at, v_at, k_cache_at, v_cache_at, block_table.data_ptr(), lengths.data_ptr(), mask_at, out.data_ptr(),
                                 0 if scratch is None else scratch.data_ptr(), nbytes, code, B, T, H, Hk, D, pages, page, width, sq[0], sq[1], sq[2], new[0], new[1], new[2],
                                 cache[0], cache[1], cache[2], block_table.stride(0), mask_batch, D ** -0.5 if scale is None else scale)
     rc = lib.i4tc_tree_attention(args, index, _raw_stream(index) if _raw_stream is not None else _stream(q))

@@ -415,16 +415,27 @@ int i4tc_qk_norm_rope(void* qkv, int64_t tokens, int64_t ld, int64_t q_heads, in
  * [G, rows, 64] with scales [G, rows]; per_channel: [rows, K/2] with [rows]), without quantising the activations:
  * exact products, fp32 sums, one rounding.  gated: W has 2 N rows and out = silu(x . W[0, N)^T) * (x . W[N, 2 N)^T).
  * Made for up to 32 tokens; more read the weights once for every 32. */
-int i4tc_w4a16_linear(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, const uint8_t* w, const float* w_scale,
-                      int per_channel, int gated, void* out, int64_t N, int device, void* stream);
+typedef struct {
+  const void* x;
+  const uint8_t* w;
+  const float* w_scale;
+  void* out;
+  int64_t dtype, M, K, ldx, N, per_channel, gated;
+} i4tc_w4a16_args;
+int i4tc_w4a16_linear(const i4tc_w4a16_args* args, int device, void* stream);
 
 /* Rotary embedding of the first R of D elements of x [tokens, heads, D] (bf16 / fp16, strides in elements, elements of a head
  * contiguous) at positions [tokens] (int32, or int64 with long_positions): a pair (a, b) becomes
  * scale * (a cos - b sin, b cos + a sin) with the angle position * freqs[i] (float64 [R/2], radians a position), minus the angle with
  * inverse.  Pairs are (i, i + R/2), interleaved: (2i, 2i + 1).  Elements behind R are copied.  out may be x (same strides). */
-int i4tc_rope(const void* x, int dtype, int64_t tokens, int64_t heads, int64_t D, int64_t R, int64_t x_token, int64_t x_head,
-              const void* positions, int long_positions, const double* freqs, int interleaved, float scale, int inverse,
-              void* out, int64_t out_token, int64_t out_head, int device, void* stream);
+typedef struct {
+  const void *x, *positions;
+  const double* freqs;
+  void* out;
+  int64_t dtype, tokens, heads, D, R, x_token, x_head, out_token, out_head, long_positions, interleaved, inverse;
+  double scale;
+} i4tc_rope_args;
+int i4tc_rope(const i4tc_rope_args* args, int device, void* stream);
 
 /* Attention of `tokens` new tokens of every sequence over its cache and over one another:
  *   q [batch, tokens, heads, D], k and v [batch, tokens, kv_heads, D], out [batch, tokens, heads, D] contiguous (bf16 / fp16);

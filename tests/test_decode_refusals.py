@@ -10,29 +10,32 @@ def _cabi(lib_built):
     return _cabi
 
 
-def test_linear(lib_built):
-    c = _cabi(lib_built)
-    call = lambda *a: c.lib.i4tc_w4a16_linear(*a, 0, None)  # noqa: E731
-    x = w = s = o = 4096                                    # addresses that nothing reads
-    for args, match in [((x, c.FP32, 1, 128, 128, w, s, 0, 0, o, 8), "bfloat16"), ((x, c.BF16, -1, 128, 128, w, s, 0, 0, o, 8), "size"),
-                        ((x, c.BF16, 1, 0, 0, w, s, 0, 0, o, 8), "size"), ((x, c.BF16, 1, 192, 192, w, s, 0, 0, o, 8), "divisible"),
-                        ((x, c.BF16, 1, 96, 96, w, s, 1, 0, o, 8), "multiple of 64"), ((x, c.BF16, 1, 1 << 21, 1 << 21, w, s, 0, 0, o, 8), "too large"),
-                        ((x + 2, c.BF16, 1, 128, 128, w, s, 0, 0, o, 8), "aligned"), ((x, c.BF16, 1, 128, 130, w, s, 0, 0, o, 8), "aligned"),
-                        ((None, c.BF16, 1, 128, 128, w, s, 0, 0, o, 8), "null")]:
-        assert call(*args) < 0 and match in c.last_error()
-    assert call(None, c.BF16, 0, 128, 128, None, None, 0, 0, None, 8) == 0
+LINEAR = dict(x=4096, w=4096, scale=4096, out=4096, dtype=0, M=1, K=128, ldx=128, N=8, per_channel=0, gated=0)   # addresses that nothing reads
 
 
-def test_rope(lib_built):
+@pytest.mark.parametrize("change,match", [
+    (dict(dtype=2), "bfloat16"), (dict(M=-1), "size"), (dict(K=0), "size"), (dict(K=192, ldx=192), "divisible"), (dict(K=96, ldx=96, per_channel=1), "multiple of 64"),
+    (dict(K=1 << 21, ldx=1 << 21), "too large"), (dict(x=4098), "aligned"), (dict(ldx=130), "aligned"), (dict(x=0), "null"),
+])
+def test_linear(lib_built, change, match):
     c = _cabi(lib_built)
-    call = lambda *a: c.lib.i4tc_rope(*a, 0, None)  # noqa: E731
-    x, at, f, o = 4096, 8192, 16384, 1 << 20
-    for args, match in [((x, c.FP32, 1, 1, 8, 8, 8, 8, at, 0, f, 0, 1.0, 0, o, 8, 8), "bfloat16"), ((x, c.BF16, 1, 1, 8, 7, 8, 8, at, 0, f, 0, 1.0, 0, o, 8, 8), "even"),
-                        ((x, c.BF16, 1, 1, 8, 10, 8, 8, at, 0, f, 0, 1.0, 0, o, 8, 8), "even"), ((x, c.BF16, 1, 1, 8, 8, 8, 8, None, 0, f, 0, 1.0, 0, o, 8, 8), "null"),
-                        ((x, c.BF16, 1, 1, 8, 8, 8, 8, at, 0, f, 0, 1.0, 0, x, 16, 8), "strides"), ((x + 1, c.BF16, 1, 1, 8, 8, 8, 8, at, 0, f, 0, 1.0, 0, o, 8, 8), "aligned"),
-                        ((x, c.BF16, 1, 1, 4096, 8, 8, 8, at, 0, f, 0, 1.0, 0, o, 8, 8), "size")]:
-        assert call(*args) < 0 and match in c.last_error()
-    assert call(None, c.BF16, 0, 1, 8, 8, 8, 8, None, 0, None, 0, 1.0, 0, None, 8, 8) == 0
+    assert c.lib.i4tc_w4a16_linear(struct.pack("@4P7q", *{**LINEAR, **change}.values()), 0, None) < 0 and match in c.last_error()
+    assert c.lib.i4tc_w4a16_linear(None, 0, None) < 0
+    assert c.lib.i4tc_w4a16_linear(struct.pack("@4P7q", *{**LINEAR, "M": 0}.values()), 0, None) == 0
+
+
+ROPE = dict(x=4096, positions=8192, freqs=16384, out=1 << 20, dtype=0, tokens=1, heads=1, D=8, R=8, xt=8, xh=8, ot=8, oh=8, long=0, inter=0, inverse=0)
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(dtype=2), "bfloat16"), (dict(R=7), "even"), (dict(R=10), "even"), (dict(positions=0), "null"), (dict(out=4096, ot=16), "strides"),
+    (dict(x=4097), "aligned"), (dict(long=1, positions=8196), "aligned"), (dict(D=4096), "size"),
+])
+def test_rope(lib_built, change, match):
+    c = _cabi(lib_built)
+    assert c.lib.i4tc_rope(struct.pack("@4P12qd", *{**ROPE, **change}.values(), 1.0), 0, None) < 0 and match in c.last_error()
+    assert c.lib.i4tc_rope(None, 0, None) < 0
+    assert c.lib.i4tc_rope(struct.pack("@4P12qd", *{**ROPE, "tokens": 0}.values(), 1.0), 0, None) == 0
 
 
 ATTENTION = ("q k v k_cache v_cache table lengths mask out scratch bytes dtype batch tokens heads kv_heads D pages page width "
