@@ -4,6 +4,7 @@
 // j lies in page block_table[b, j / page_size], row j % page_size.
 #include "common.cuh"
 #include "ptx.cuh"
+#include <float.h>
 #include <math.h>
 #include <math_constants.h>
 #include <type_traits>
@@ -935,6 +936,7 @@ extern "C" int i4tc_tree_attention(const i4tc_tree_attention_args* a, int device
   I4TC_REQUIRE(a->kv_heads > 0 && a->heads % a->kv_heads == 0 && a->heads <= 65536, I4TC_EINVAL, "heads must be a multiple of kv_heads");
   I4TC_REQUIRE(a->batch <= 65536 && a->pages >= 0 && a->pages < (1ll << 31) && a->page_size > 0 && a->page_size < (1ll << 31) &&
                    a->table_width >= 0 && a->table_width < (1ll << 31), I4TC_EINVAL, "bad size");
+  I4TC_REQUIRE(isfinite(a->scale) && fabs(a->scale) < 1e30, I4TC_EINVAL, "the scale must be finite");
   I4TC_REQUIRE(a->q && a->k && a->v && a->lengths && a->out, I4TC_EINVAL, "null pointer");
   I4TC_REQUIRE(a->table_width == 0 || a->pages == 0 || (a->k_cache && a->v_cache && a->block_table), I4TC_EINVAL, "null pointer");
   I4TC_REQUIRE(aligned_to(a->k, 16) && aligned_to(a->v, 16) && aligned_to(a->k_cache, 16) && aligned_to(a->v_cache, 16) &&
@@ -967,7 +969,7 @@ extern "C" int i4tc_tree_attention(const i4tc_tree_attention_args* a, int device
   I4TC_REQUIRE(p.ranks || a->scratch != nullptr, I4TC_EINVAL, "null pointer");
   I4TC_REQUIRE(p.ranks || a->scratch_bytes >= (int64_t)p.parts * p.lines * 2 * (int64_t)slot_floats(16 * warps, padded_dim(p.D)) * 4, I4TC_EWORKSPACE,
                "the scratch is too small");
-  p.scale_log2 = fmaxf((float)(fabs(a->scale) * 1.4426950408889634), 1e-30f);
+  p.scale_log2 = fmaxf((float)(fabs(a->scale) * 1.4426950408889634), FLT_MIN);
   p.flip = a->scale < 0 ? 0x80008000u : 0u;
   p.status = info->status;
   DeviceGuard guard(device);

@@ -553,7 +553,7 @@ extern "C" int i4tc_w4a16_linear(const i4tc_w4a16_args* a, int device, void* str
       }
     }
   }
-  I4TC_REQUIRE(grid_x > 0, I4TC_EUNSUPPORTED, "K is too large");
+  I4TC_REQUIRE(grid_x > 0 && chunks <= 65535, I4TC_EUNSUPPORTED, "K is too large, or there are too many tokens for it");
   const size_t smem = w4a16_smem(tokens, small, p.units_each, (p.tiles + grid_x - 1) / grid_x, kWarps / p.tile_warps);
   const dim3 grid((unsigned)grid_x, (unsigned)p.ranks, (unsigned)chunks);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

@@ -44,6 +44,12 @@ GOOD = dict(q=4096, k=4096, v=4096, k_cache=4096, v_cache=4096, table=4096, leng
             heads=2, kv_heads=1, D=64, pages=4, page=16, width=4, qb=128, qt=128, qh=64, nb=64, nt=64, nh=64, ps=1024, ss=64, hs=64, ts=4, mb=0)
 
 
+@pytest.mark.parametrize("scale", [float("nan"), float("inf"), -float("inf")])
+def test_attention_scale(lib_built, scale):
+    c = _cabi(lib_built)
+    assert c.lib.i4tc_tree_attention(struct.pack("@10P21qd", *GOOD.values(), scale), 0, None) < 0 and "finite" in c.last_error()
+
+
 @pytest.mark.parametrize("change,match", [
     (dict(dtype=2), "bfloat16"), (dict(batch=-1), "size"), (dict(tokens=65), "64 new"), (dict(D=136), "128 elements"), (dict(D=12), "multiple of 8"),
     (dict(kv_heads=0), "multiple of kv_heads"), (dict(heads=3, kv_heads=2), "multiple of kv_heads"), (dict(page=0), "size"), (dict(q=0), "null"),

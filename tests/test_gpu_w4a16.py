@@ -73,18 +73,20 @@ def test_gated(M, K, I, per_channel, dtype):
     _check(out, act * u, 1.1 * dg * u.abs() + act.abs() * du + 1.1 * dg * du + (16 + g.abs()) * 2.0 ** -23 * (act * u).abs())
 
 
-def test_linear_equals_its_tokens_one_by_one():
-    """Padding tokens and the tokens of other grid rows have no part in a token's sums."""
+def test_tokens_do_not_mix():
+    """Padding tokens and the tokens of other grid rows have no part in a token's sums: finite ones beside NaN and infinity, and each by itself."""
     from fp8_inference_toolkit_b200 import ops
 
     gen = torch.Generator(device="cuda").manual_seed(5)
     x = torch.randn(37, 1024, device="cuda", generator=gen).to(torch.bfloat16)
     x[3], x[20] = float("nan"), float("inf")
-    packed, scale, _ = _weights(gen, 77, 1024, False)
+    packed, scale, w = _weights(gen, 77, 1024, False)
     whole = ops.w4a16_linear(x, packed, scale, 77)
-    for m in range(37):
-        assert torch.equal(ops.w4a16_linear(x[m:m + 1], packed, scale, 77)[0].nan_to_num(7.0), whole[m].nan_to_num(7.0))
-    assert whole[3].isnan().all() and not whole[20].isfinite().any()
+    single = torch.cat([ops.w4a16_linear(x[m:m + 1], packed, scale, 77) for m in range(37)])
+    fine = [m for m in range(37) if m not in (3, 20)]
+    for out in (whole, single):
+        _check(out[fine], *_product(x[fine], w))
+        assert out[3].isnan().all() and not out[20].isfinite().any()
 
 
 @pytest.mark.parametrize("gated", [False, True])
