@@ -127,7 +127,7 @@ struct AttendParams {
   int parts;                    // of the line, at most
   int ranks;                    // blocks of a cluster, where a sequence has its own; else 0
   float scale_log2;             // |scale| * log2(e), not zero: what is masked stays so
-  uint32_t flip;                // sign bits of two queries, where the scale is negative
+  int negative;                 // the scale's sign
   unsigned int* status;
 };
 
@@ -324,6 +324,36 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
   }
   Cursor ahead = cur;                               // whose places are looked up next
 
+  uint32_t q[KS][4];
+  float o[DT][4], m[2], l[4];                       // m: reference of the weights, not yet scaled; l: sums of the weights (rows g, and 8 + g from l[2])
+  int tok[2];                                       // of this lane's two rows; -1 behind the last
+  // The item's queries and running state.
+  auto begin = [&]() {
+    const int row0 = tile_row0 + wr * 16 + g;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const int row = row0 + 8 * h;
+      tok[h] = row < p.rows ? row / p.group : -1;
+      const T* src = static_cast<const T*>(p.q) + cur.b * p.q_batch + (long long)(row / p.group) * p.q_token +
+                     (long long)(kvh * p.group + row % p.group) * p.q_head;
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int d = ks * 16 + e * 8 + 2 * t4;
+          q[ks][2 * e + h] = tok[h] >= 0 && d < p.D ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
+        }
+      m[h] = -CUDART_INF_F;
+      l[2 * h] = l[2 * h + 1] = 0.f;
+    }
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[dt][k] = 0.f;
+  };
+  // Before the first tiles: behind their copies the queries came 5 us later (all blocks ask for 19 MB then).
+  begin();
+
   // Places of the tile at `ahead`: key tid of it.  In two halves, the page's number and the addresses, so that nobody waits for the table.
   // Where there is no place (behind the new tokens, pages out of range) some row that exists.
   auto look_up = [&](const Cursor& ahead) -> int {
@@ -386,9 +416,6 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
   }
   int next_rows = rows[kStages - 1];                // of the tile to be issued next
 
-  uint32_t q[KS][4];
-  float o[DT][4], m[2], l[4];                       // m: reference of the weights, not yet scaled; l: sums of the weights (rows g, and 8 + g from l[2])
-  int tok[2];                                       // of this lane's two rows; -1 behind the last
   // Where this lane reads a tile's keys and values for ldmatrix: chunk c of a row stands at c ^ (row & 7), so chunks 2 j + {0, 1} of eight
   // are four addresses, and the rest (other rows, the next eight chunks) is added to them.
   const int key0 = wk * S::KEYS;                    // this warp's keys in a tile
@@ -401,31 +428,6 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
   }
   bool whole = cur.tile == 0;                       // this part has the item from its start
 
-  // The item's queries and running state.
-  auto begin = [&]() {
-    const int row0 = tile_row0 + wr * 16 + g;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int row = row0 + 8 * h;
-      tok[h] = row < p.rows ? row / p.group : -1;
-      const T* src = static_cast<const T*>(p.q) + cur.b * p.q_batch + (long long)(row / p.group) * p.q_token +
-                     (long long)(kvh * p.group + row % p.group) * p.q_head;
-#pragma unroll
-      for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int d = ks * 16 + e * 8 + 2 * t4;
-          q[ks][2 * e + h] = tok[h] >= 0 && d < p.D ? *reinterpret_cast<const uint32_t*>(src + d) ^ p.flip : 0u;
-        }
-      m[h] = -CUDART_INF_F;
-      l[2 * h] = l[2 * h + 1] = 0.f;
-    }
-#pragma unroll
-    for (int dt = 0; dt < DT; ++dt)
-#pragma unroll
-      for (int k = 0; k < 4; ++k) o[dt][k] = 0.f;
-  };
-  begin();                                          // (its loads under the first tiles' copies)
   int stage = 0;                                    // of tile i
   for (int i = 0; i < count; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
@@ -453,6 +455,12 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
         mma<T>(s[2 * np], q[ks], b[0], b[1]);
         mma<T>(s[2 * np + 1], q[ks], b[2], b[3]);
       }
+    if (p.negative) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) s[nt][k] = -s[nt][k];
+    }
     const int j0 = cur.tile * kTile;
     const bool edge = j0 + kTile > cur.length;      // the tile holds new tokens, or what is behind them
     bool odd = false;
@@ -970,7 +978,7 @@ extern "C" int i4tc_tree_attention(const i4tc_tree_attention_args* a, int device
   I4TC_REQUIRE(p.ranks || a->scratch_bytes >= (int64_t)p.parts * p.lines * 2 * (int64_t)slot_floats(16 * warps, padded_dim(p.D)) * 4, I4TC_EWORKSPACE,
                "the scratch is too small");
   p.scale_log2 = fmaxf((float)(fabs(a->scale) * 1.4426950408889634), FLT_MIN);
-  p.flip = a->scale < 0 ? 0x80008000u : 0u;
+  p.negative = a->scale < 0;
   p.status = info->status;
   DeviceGuard guard(device);
   I4TC_CUDA(guard.err);
