@@ -327,22 +327,30 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
   uint32_t q[KS][4];
   float o[DT][4], m[2], l[4];                       // m: reference of the weights, not yet scaled; l: sums of the weights (rows g, and 8 + g from l[2])
   int tok[2];                                       // of this lane's two rows; -1 behind the last
-  // The item's queries and running state.
-  auto begin = [&]() {
-    const int row0 = tile_row0 + wr * 16 + g;
+  // This lane's rows are the same for every sequence; its queries of sequence b, and a sequence's running state.
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int row = tile_row0 + wr * 16 + g + 8 * h;
+    tok[h] = row < p.rows ? row / p.group : -1;
+  }
+  auto load_queries = [&](int b, uint32_t (&to)[KS][4]) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const int row = row0 + 8 * h;
-      tok[h] = row < p.rows ? row / p.group : -1;
-      const T* src = static_cast<const T*>(p.q) + cur.b * p.q_batch + (long long)(row / p.group) * p.q_token +
+      const int row = tile_row0 + wr * 16 + g + 8 * h;
+      const T* src = static_cast<const T*>(p.q) + b * p.q_batch + (long long)(row / p.group) * p.q_token +
                      (long long)(kvh * p.group + row % p.group) * p.q_head;
 #pragma unroll
       for (int ks = 0; ks < KS; ++ks)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           const int d = ks * 16 + e * 8 + 2 * t4;
-          q[ks][2 * e + h] = tok[h] >= 0 && d < p.D ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
+          to[ks][2 * e + h] = tok[h] >= 0 && d < p.D ? *reinterpret_cast<const uint32_t*>(src + d) : 0u;
         }
+    }
+  };
+  auto begin = [&]() {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
       m[h] = -CUDART_INF_F;
       l[2 * h] = l[2 * h + 1] = 0.f;
     }
@@ -352,6 +360,7 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
       for (int k = 0; k < 4; ++k) o[dt][k] = 0.f;
   };
   // Before the first tiles: behind their copies the queries came 5 us later (all blocks ask for 19 MB then).
+  load_queries(cur.b, q);
   begin();
 
   // Places of the tile at `ahead`: key tid of it.  In two halves, the page's number and the addresses, so that nobody waits for the table.
@@ -429,6 +438,8 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
   bool whole = cur.tile == 0;                       // this part has the item from its start
 
   int stage = 0;                                    // of tile i
+  uint32_t next_q[KS][4] = {};
+  bool asked = false;
   for (int i = 0; i < count; ++i) {
     asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
     __syncthreads();
@@ -438,6 +449,11 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
     int page = 0;
     if (more && tid < kTile) page = look_up(ahead);
     next_rows = ahead.length + p.tokens - ahead.tile * kTile;
+    // the next sequence's queries, two tiles before they are wanted: among the copies they take microseconds
+    if (!OWN && !asked && cur.tile + 3 >= cur.tiles && i + cur.tiles - cur.tile < count) {
+      load_queries(cur.b + 1, next_q);
+      asked = true;
+    }
 
     const uint32_t at_stage = stage * 2 * S::kStage, sv = stage0 + at_stage + S::kStage;
     if (++stage == kStages) stage = 0;
@@ -662,7 +678,14 @@ __global__ void __launch_bounds__(kAttendThreads) attend_kernel(const AttendPara
     }
     const bool another = !OWN && ends && i + 1 < count;
     cur.next<OWN>(p, line);
-    if (another) begin();
+    if (another) {
+#pragma unroll
+      for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) q[ks][k] = next_q[ks][k];
+      begin();
+      asked = false;
+    }
     if (more) {
       if (tid < kTile) places[((i + kStages) % kPlaces) * kTile + tid] = place_of(ahead, page);
       ahead.next<OWN>(p, line);
