@@ -110,7 +110,7 @@ __device__ __forceinline__ uint32_t codes_pair(uint32_t w, uint32_t bias) {
 __device__ __forceinline__ void store_as(__nv_bfloat16* p, float v) { *p = __float2bfloat16_rn(v); }
 __device__ __forceinline__ void store_as(__half* p, float v) { *p = __float2half_rn(v); }
 
-constexpr int token_tiles(int tokens, bool small) { return small || tokens > 16 ? 4 : tokens > 8 ? 2 : 1; }
+constexpr int token_tiles(int tokens, bool small) { return small || tokens > 24 ? 4 : (tokens + 7) / 8; }
 constexpr int ring_depth(int token_tiles) { return token_tiles == 1 ? 8 : 4; }
 constexpr size_t w4a16_smem(int tokens, bool small, int units_each, int block_tiles, int k_warps) {
   return (size_t)units_each * tokens * 256                              // the tokens
@@ -388,16 +388,21 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_kernel(const W4A16Params p)
   const uint32_t base = ptx::smem_u32(part);
   for (int i = rank * share + threadIdx.x; i < min(values, (rank + 1) * share); i += kThreads) {
     const int r = i % COLS, q = i / COLS, tile = q / M, m = q - tile * M, at = (tile * k_warps * M + m) * 16 + r;
-    float v = 0.f, up = 0.f;
-    for (int k = 0; k < p.ranks; ++k) {
-      const uint32_t from = ptx::mapa_shared(base, k) + 4u * at;
-      float a;
-      asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(a) : "r"(from));
-      v += a;
-      if constexpr (GATED) {
-        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(a) : "r"(from + 32u));
-        up += a;
+    float of[8], of_up[8];                                                // all on their way before the first is added
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      of[k] = of_up[k] = 0.f;
+      if (k < p.ranks) {
+        const uint32_t from = ptx::mapa_shared(base, k) + 4u * at;
+        asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(of[k]) : "r"(from));
+        if constexpr (GATED) asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(of_up[k]) : "r"(from + 32u));
       }
+    }
+    float v = 0.f, up = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      v += of[k];
+      up += of_up[k];
     }
     finish(tile, m, r, v, up);
   }
@@ -469,6 +474,7 @@ int launch_tokens(const W4A16Params& p, dim3 grid, size_t smem, cudaStream_t st)
   switch (token_tiles(p.M < p.most_tokens ? p.M : p.most_tokens, false)) {
     case 1: return launch_one<T, 1, GATED, ROWMAJOR, false>(p, grid, smem, st);
     case 2: return launch_one<T, 2, GATED, ROWMAJOR, false>(p, grid, smem, st);
+    case 3: return launch_one<T, 3, GATED, ROWMAJOR, false>(p, grid, smem, st);
     default: return launch_one<T, 4, GATED, ROWMAJOR, false>(p, grid, smem, st);
   }
 }
@@ -541,7 +547,7 @@ extern "C" int i4tc_w4a16_linear(const i4tc_w4a16_args* a, int device, void* str
       const int warp_steps = (block_tiles + tw - 1) / tw * steps;
       // Microseconds: a step of a block costs its instructions, or a warp's steps their latency; the tokens' rows are laid out by
       // every block; sums are added per warp that splits K, and between the ranks of a cluster.
-      const double issue = (0.8 * block_tiles * each + 0.2 * kWarps * warp_steps) * (nt == 1 ? 0.033 : nt == 2 ? 0.05 : 0.098);
+      const double issue = (0.8 * block_tiles * each + 0.2 * kWarps * warp_steps) * (nt == 1 ? 0.033 : nt == 2 ? 0.05 : nt == 3 ? 0.074 : 0.098);
       const double latency = warp_steps * 0.35;
       const double layout = each * tokens * (nt == 1 ? 0.011 : 0.006);
       const double sums = (double)block_tiles * tokens * 16 * (k_warps - 1) * 0.0005;
