@@ -188,26 +188,51 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_kernel(const W4A16Params p)
     }
   };
   aim();
-#pragma unroll
-  for (int d = 0; d < DEPTH; ++d) {
-    if (d < total) fetch(d);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
+  auto fill = [&]() {
+#pragma unroll 1
+    for (int d = 0; d < DEPTH; ++d) {
+      if (d < total) fetch(d);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  };
 
   // The tokens, as the operand of the instruction: 16 bytes = eight numbers of one token in pairs (i, i + 4).  Sixteen lanes have a token's
-  // numbers of a unit.  PLAIN: as they are.  Returns whether a number would not stay exact.
-  auto lay_out = [&](auto plain) {
+  // numbers of a unit.  They are asked for before the weights, which all blocks ask for by the megabyte: behind those the sixteen tokens
+  // of K 12288 came 4 us later.
+  constexpr int BATCH = 8;                                                // passes whose loads are on their way together
+  const int chunk = threadIdx.x & 15, passes = (units * M + kThreads / 16 - 1) / (kThreads / 16);
+  struct Row {
+    int u, m;
+  };
+  const int step_m = kThreads / 16 / units, step_u = kThreads / 16 - step_m * units;
+  auto first_row = [&]() {
+    const int r = threadIdx.x >> 4;
+    return Row{r % units, r / units};
+  };
+  auto advance = [&](Row& r) {
+    r.u += step_u;
+    r.m += step_m;
+    if (r.u >= units) { r.u -= units; ++r.m; }
+  };
+  auto load = [&](uint4 (&v)[BATCH], Row& at, int count) {
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      v[j] = make_uint4(0u, 0u, 0u, 0u);
+      if (j >= count) continue;
+      const int k = (u0 + at.u) * 128 + chunk * 8;
+      if (at.m < M && k < p.K) v[j] = __ldg(reinterpret_cast<const uint4*>(x + (long long)(m0 + at.m) * p.ldx + k));
+      advance(at);
+    }
+  };
+  // PLAIN: as they are.  Returns whether a number would not stay exact.
+  auto keep = [&](const uint4 (&of)[BATCH], Row& at, int count, auto plain) {
     constexpr bool PLAIN = decltype(plain)::value;
     bool lost = false;
-    const int c = threadIdx.x & 15;                                       // 16 bytes of the 256
-    int u = threadIdx.x >> 4, m = 0;
-    while (u >= units) { u -= units; ++m; }
-#pragma unroll 2
-    for (int i0 = 0; i0 < units * M; i0 += kThreads / 16) {
-      const int k = (u0 + u) * 128 + c * 8;
-      const bool in = m < M;
-      uint4 v = make_uint4(0u, 0u, 0u, 0u);
-      if (in && k < p.K) v = __ldg(reinterpret_cast<const uint4*>(x + (long long)(m0 + m) * p.ldx + k));
+#pragma unroll
+    for (int j = 0; j < BATCH; ++j) {
+      if (j >= count) break;
+      const uint4 v = of[j];
+      const bool in = at.m < M;
       uint4 r = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
       if constexpr (!PLAIN) {
         uint32_t top = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
@@ -215,10 +240,10 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_kernel(const W4A16Params p)
         uint32_t* pair = &r.x;
         float lo[4], hi[4], sum = 0.f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          lo[j] = to_f32(reinterpret_cast<const T*>(pair + j)[0]);
-          hi[j] = to_f32(reinterpret_cast<const T*>(pair + j)[1]);
-          sum += lo[j] + hi[j];
+        for (int k = 0; k < 4; ++k) {
+          lo[k] = to_f32(reinterpret_cast<const T*>(pair + k)[0]);
+          hi[k] = to_f32(reinterpret_cast<const T*>(pair + k)[1]);
+          sum += lo[k] + hi[k];
         }
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) {
@@ -230,26 +255,40 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_kernel(const W4A16Params p)
         lost |= e == Bits<T>::kTop || up < -100;
         const float f = __uint_as_float((uint32_t)(127 + up) << 23), back = __uint_as_float((uint32_t)(127 - up) << 23);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const float fj = j & 1 ? f * 0.0625f : f, bj = j & 1 ? back * 16.0f : back;
-          const __half2 h = __floats2half2_rn(lo[j] * fj, hi[j] * fj);
+        for (int k = 0; k < 4; ++k) {
+          const float fk = k & 1 ? f * 0.0625f : f, bk = k & 1 ? back * 16.0f : back;
+          const __half2 h = __floats2half2_rn(lo[k] * fk, hi[k] * fk);
           const float2 again = __half22float2(h);
-          lost |= again.x * bj != lo[j] || again.y * bj != hi[j];
-          pair[j] = *reinterpret_cast<const uint32_t*>(&h);
+          lost |= again.x * bk != lo[k] || again.y * bk != hi[k];
+          pair[k] = *reinterpret_cast<const uint32_t*>(&h);
         }
-        if (in && c == 0) ab[u * 8 * NT + m] = make_float2(back * 16777216.0f, 8.0f * sum);
+        if (in && chunk == 0) ab[at.u * 8 * NT + at.m] = make_float2(back * 16777216.0f, 8.0f * sum);
       }
-      if (in) xs[(u * M + m) * 16 + ((c & 3) ^ (m & 1)) * 4 + (c >> 2)] = r;
-      u += kThreads / 16;
-      while (u >= units) { u -= units; ++m; }
+      if (in) xs[(at.u * M + at.m) * 16 + ((chunk & 3) ^ (at.m & 1)) * 4 + (chunk >> 2)] = r;
+      advance(at);
     }
+    return lost;
+  };
+  auto lay_out = [&](auto plain, bool with_weights) {
+    uint4 v[BATCH];
+    Row loaded = first_row(), kept = loaded;
+    bool lost = false;
+    int q = 0;
+#pragma unroll 1
+    for (; q + BATCH < passes; q += BATCH) {
+      load(v, loaded, BATCH);
+      lost |= keep(v, kept, BATCH, plain);
+    }
+    load(v, loaded, passes - q);
+    if (with_weights) fill();
+    lost |= keep(v, kept, passes - q, plain);
     return lost;
   };
   // (with more than eight tokens the scaling of all of them costs more than it saves: the tensor instructions bound the walk)
   bool plain = true;
-  if constexpr (NT == 1) plain = __syncthreads_or(lay_out(std::false_type{}));
+  if constexpr (NT == 1) plain = __syncthreads_or(lay_out(std::false_type{}, true));
   if (plain) {
-    lay_out(std::true_type{});
+    lay_out(std::true_type{}, NT != 1);
     __syncthreads();
   }
 
