@@ -29,8 +29,8 @@
 // laying them out in every block costs more than adding up; its partial sums are added in ascending order through distributed
 // shared memory: no workspace, no second launch, and the same bits in every run.
 //
-// Measured (device time, weights from HBM, bf16, per-group scales): [1, 4096] x [6144, 4096] 5.7 us, [16, 12288] x [4096, 12288]
-// 18.1, gated [1, 4096] x [24576, 4096] 14.9 (3.6 TB/s), [16, ...] 22.7, [32, ...] 42.
+// Measured (device time, weights from HBM, bf16, per-group scales): [1, 4096] x [6144, 4096] 6.2 us, [16, 12288] x [4096, 12288]
+// 14.5, gated [1, 4096] x [24576, 4096] 14.9 (3.6 TB/s; 5.5 between start and end), [16, ...] 21.9, [32, ...] 37.7.
 #include "common.cuh"
 #include "ptx.cuh"
 #include <type_traits>
