@@ -10,17 +10,14 @@
 // A block (sixteen warps, one an SM) takes a contiguous range of 16-row tiles, so that every SM has the same share whatever N is.
 // Its warps take the tiles in turn, split K, or both.  A step is one tile's 128 codes of K (1 KB) and their scales, which a lane
 // copies for itself into a ring of the warp's, up to eight steps ahead, by cp.async: no registers and no barrier, and no waiting on
-// loads issued later (with the ring in registers the six scoreboards of a warp were shared between its steps: 19.5 us instead
-// of 14.9 for the gated [1, 4096] x [24576, 4096]; bulk copies on mbarriers cost 80 instructions a step).
+// loads issued later (with the ring in registers the six scoreboards of a warp were shared between its steps, which cost the gated
+// [1, 4096] x [24576, 4096] 4.6 us; bulk copies on mbarriers cost 80 instructions a step).
 //
-// Codes become operands by one masking instruction each (and a shift for every second pair): a nibble in the low bits of a 16-bit
-// word, its top bit flipped, is the fp16 subnormal (code + 8) * 2^-24, one bit group further up (code + 8) * 2^-20.  The
-// tokens meet them as fp16 too: the 128 numbers of a step are scaled by the power of two that brings the largest to 2^15 (a
-// sixteenth of that where they meet the upper nibbles), which is exact for all that are not 2^28 times smaller, and 8 times their sum
-// comes off the result.  Products are exact and sums fp32 as they would be with codes and tokens themselves; the +8 makes their terms
-// three times larger.  Where a number would not stay exact, or is infinite or none, the block takes the plain way: codes as numbers
-// of the tokens' type (128 + 8 or 1024 + 8 taken off by a subtraction), tokens as they are.  So do more than eight tokens, for
-// which the tensor instructions bound the walk.
+// Codes become operands of the tokens' type by masking and a subtraction: a nibble with its top bit flipped, in the low bits of the
+// number 128 (bf16) or 1024 (fp16), is that number + 8 + code, and the difference is exact.  So are the products, and the fp32 sums hold
+// nothing but the formula's terms: where a code is zero, the token's number has no part, however large.  (Leaving the +8 in and taking 8
+// times the tokens' sum off the result saves the subtraction, 14.9 us instead of 16.4 for one gated token, but a number
+// 2^20 times as large as the others then costs their sums 20 bits wherever its code is zero.)
 //
 // The k order inside an instruction is free as long as both operands agree: a word's nibbles come out as pairs (i, i + 4), and the
 // tokens are laid out in these pairs, once, in shared memory.
@@ -29,8 +26,8 @@
 // laying them out in every block costs more than adding up; its partial sums are added in ascending order through distributed
 // shared memory: no workspace, no second launch, and the same bits in every run.
 //
-// Measured (device time, weights from HBM, bf16, per-group scales): [1, 4096] x [6144, 4096] 6.2 us, [16, 12288] x [4096, 12288]
-// 14.5, gated [1, 4096] x [24576, 4096] 14.9 (3.6 TB/s; 5.5 between start and end), [16, ...] 21.9, [32, ...] 37.7.
+// Measured (device time, weights from HBM, bf16, per-group scales): [1, 4096] x [6144, 4096] 6.5 us, [16, 12288] x [4096, 12288]
+// 14.4, gated [1, 4096] x [24576, 4096] 16.4 (3.3 TB/s), [16, ...] 21.7, [32, ...] 37.3.
 #include "common.cuh"
 #include "ptx.cuh"
 #include <type_traits>
@@ -114,14 +111,9 @@ constexpr int token_tiles(int tokens, bool small) { return small || tokens > 24 
 constexpr int ring_depth(int token_tiles) { return token_tiles == 1 ? 8 : 4; }
 constexpr size_t w4a16_smem(int tokens, bool small, int units_each, int block_tiles, int k_warps) {
   return (size_t)units_each * tokens * 256                              // the tokens
-         + (size_t)units_each * token_tiles(tokens, small) * 64         // factor and offset of each in a step
          + (size_t)block_tiles * k_warps * tokens * 64                  // partial sums
          + (size_t)kWarps * ring_depth(token_tiles(tokens, small)) * kStep;   // rings
 }
-
-template <typename T> struct Bits;   // of the tokens' type: exponent's place, bias and highest value
-template <> struct Bits<__nv_bfloat16> { static constexpr int kShift = 7, kBias = 127, kTop = 255; };
-template <> struct Bits<__half> { static constexpr int kShift = 10, kBias = 15, kTop = 31; };
 
 // NT: 8-token tiles.  GATED: a tile's sixteen rows are eight columns' gate rows and then their up rows.  ROWMAJOR: codes [rows, K / 2]
 // and one scale a row, else [units, rows, 64] and a scale for each unit.  SMALL: fewer columns than a tile has.
@@ -138,8 +130,7 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_kernel(const W4A16Params p)
   const int wn = warp % p.tile_warps, wk = warp / p.tile_warps, k_warps = kWarps / p.tile_warps;
   const int first = min(units, wk * p.steps), mine = min(units, first + p.steps) - first;   // of the block's units, this warp's
   uint4* xs = reinterpret_cast<uint4*>(smem);                             // [unit][token][word][t], words of odd tokens swapped in pairs
-  float2* ab = reinterpret_cast<float2*>(xs + (size_t)p.units_each * M * 16);   // [unit][8 NT]: factor of a token's sums, and what comes off
-  uint8_t* rings = reinterpret_cast<uint8_t*>(ab + p.units_each * 8 * NT);      // [warp][slot][16 rows of codes, 16 scales]
+  uint8_t* rings = reinterpret_cast<uint8_t*>(xs + (size_t)p.units_each * M * 16);   // [warp][slot][16 rows of codes, 16 scales]
   float* part = reinterpret_cast<float*>(rings + kWarps * DEPTH * kStep); // [tile][k warp][token][16]
   const uint32_t ring = ptx::smem_u32(rings) + warp * DEPTH * kStep, ring_lane = ring + lane * 16;
 
@@ -188,13 +179,6 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_kernel(const W4A16Params p)
     }
   };
   aim();
-  auto fill = [&]() {
-#pragma unroll 1
-    for (int d = 0; d < DEPTH; ++d) {
-      if (d < total) fetch(d);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
-  };
 
   // The tokens, as the operand of the instruction: 16 bytes = eight numbers of one token in pairs (i, i + 4).  Sixteen lanes have a token's
   // numbers of a unit.  They are asked for before the weights, which all blocks ask for by the megabyte: behind those the sixteen tokens
@@ -205,10 +189,6 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_kernel(const W4A16Params p)
     int u, m;
   };
   const int step_m = kThreads / 16 / units, step_u = kThreads / 16 - step_m * units;
-  auto first_row = [&]() {
-    const int r = threadIdx.x >> 4;
-    return Row{r % units, r / units};
-  };
   auto advance = [&](Row& r) {
     r.u += step_u;
     r.m += step_m;
@@ -224,73 +204,32 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_kernel(const W4A16Params p)
       advance(at);
     }
   };
-  // PLAIN: as they are.  Returns whether a number would not stay exact.
-  auto keep = [&](const uint4 (&of)[BATCH], Row& at, int count, auto plain) {
-    constexpr bool PLAIN = decltype(plain)::value;
-    bool lost = false;
+  auto keep = [&](const uint4 (&v)[BATCH], Row& at, int count) {
 #pragma unroll
     for (int j = 0; j < BATCH; ++j) {
       if (j >= count) break;
-      const uint4 v = of[j];
-      const bool in = at.m < M;
-      uint4 r = make_uint4(__byte_perm(v.x, v.z, 0x5410), __byte_perm(v.x, v.z, 0x7632), __byte_perm(v.y, v.w, 0x5410), __byte_perm(v.y, v.w, 0x7632));
-      if constexpr (!PLAIN) {
-        uint32_t top = __vmaxu2(__vmaxu2(v.x & 0x7FFF7FFFu, v.y & 0x7FFF7FFFu), __vmaxu2(v.z & 0x7FFF7FFFu, v.w & 0x7FFF7FFFu));
-        top = max(top & 0xFFFFu, top >> 16);
-        uint32_t* pair = &r.x;
-        float lo[4], hi[4], sum = 0.f;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          lo[k] = to_f32(reinterpret_cast<const T*>(pair + k)[0]);
-          hi[k] = to_f32(reinterpret_cast<const T*>(pair + k)[1]);
-          sum += lo[k] + hi[k];
-        }
-#pragma unroll
-        for (int o = 8; o > 0; o >>= 1) {
-          top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-          sum += __shfl_xor_sync(0xffffffffu, sum, o);
-        }
-        const int e = top >> Bits<T>::kShift;
-        const int up = min(15 + Bits<T>::kBias - max(e, 1), 120);         // times 2^up
-        lost |= e == Bits<T>::kTop || up < -100;
-        const float f = __uint_as_float((uint32_t)(127 + up) << 23), back = __uint_as_float((uint32_t)(127 - up) << 23);
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float fk = k & 1 ? f * 0.0625f : f, bk = k & 1 ? back * 16.0f : back;
-          const __half2 h = __floats2half2_rn(lo[k] * fk, hi[k] * fk);
-          const float2 again = __half22float2(h);
-          lost |= again.x * bk != lo[k] || again.y * bk != hi[k];
-          pair[k] = *reinterpret_cast<const uint32_t*>(&h);
-        }
-        if (in && chunk == 0) ab[at.u * 8 * NT + at.m] = make_float2(back * 16777216.0f, 8.0f * sum);
-      }
-      if (in) xs[(at.u * M + at.m) * 16 + ((chunk & 3) ^ (at.m & 1)) * 4 + (chunk >> 2)] = r;
+      if (at.m < M)
+        xs[(at.u * M + at.m) * 16 + ((chunk & 3) ^ (at.m & 1)) * 4 + (chunk >> 2)] = make_uint4(
+            __byte_perm(v[j].x, v[j].z, 0x5410), __byte_perm(v[j].x, v[j].z, 0x7632), __byte_perm(v[j].y, v[j].w, 0x5410), __byte_perm(v[j].y, v[j].w, 0x7632));
       advance(at);
     }
-    return lost;
   };
-  auto lay_out = [&](auto plain, bool with_weights) {
-    uint4 v[BATCH];
-    Row loaded = first_row(), kept = loaded;
-    bool lost = false;
-    int q = 0;
+  uint4 held[BATCH];
+  Row loaded = {(int)(threadIdx.x >> 4) % units, (int)(threadIdx.x >> 4) / units}, kept = loaded;
+  int laid_out = 0;
 #pragma unroll 1
-    for (; q + BATCH < passes; q += BATCH) {
-      load(v, loaded, BATCH);
-      lost |= keep(v, kept, BATCH, plain);
-    }
-    load(v, loaded, passes - q);
-    if (with_weights) fill();
-    lost |= keep(v, kept, passes - q, plain);
-    return lost;
-  };
-  // (with more than eight tokens the scaling of all of them costs more than it saves: the tensor instructions bound the walk)
-  bool plain = true;
-  if constexpr (NT == 1) plain = __syncthreads_or(lay_out(std::false_type{}, true));
-  if (plain) {
-    lay_out(std::true_type{}, NT != 1);
-    __syncthreads();
+  for (; laid_out + BATCH < passes; laid_out += BATCH) {
+    load(held, loaded, BATCH);
+    keep(held, kept, BATCH);
   }
+  load(held, loaded, passes - laid_out);
+#pragma unroll 1
+  for (int d = 0; d < DEPTH; ++d) {
+    if (d < total) fetch(d);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  }
+  keep(held, kept, passes - laid_out);
+  __syncthreads();
 
   // a lane without a token of its own reads the last one: its column of the result goes nowhere
   uint32_t b_at[NT];
@@ -299,96 +238,70 @@ __global__ void __launch_bounds__(kThreads, 1) w4a16_kernel(const W4A16Params p)
     const int m = min(8 * nt + g, M - 1);
     b_at[nt] = ptx::smem_u32(xs) + (m * 16 + (m & 1) * 4 + t) * 16;
   }
-  auto walk = [&](auto plain_way) {
-    constexpr bool PLAIN = decltype(plain_way)::value;
-    // 128 + 8 in bf16 or 1024 + 8 in fp16, twice; the sign bits of the codes in either place
-    const uint32_t bias = opaque<std::is_same_v<T, __nv_bfloat16> ? 0x43084308u : 0x64086408u>();
-    const uint32_t flip_lo = opaque<0x00080008u>(), flip_hi = opaque<0x00800080u>();
-    float f[NT][4];
+  // 128 + 8 in bf16 or 1024 + 8 in fp16, twice
+  const uint32_t bias = opaque<std::is_same_v<T, __nv_bfloat16> ? 0x43084308u : 0x64086408u>();
+  float f[NT][4];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) f[nt][i] = 0.f;
+  uint32_t b_off = first * M * 256;
+  int u = 0, tile = wn;
+  int slot = 0;
+  for (int i = 0; i < total; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
+    __syncwarp();
+    const uint32_t from = ring_lane + slot * kStep;
+    const uint4 v0 = ptx::lds128(from), v1 = ptx::lds128(from + 512);
+    float s0 = 1.0f, s1 = 1.0f;
+    if constexpr (!ROWMAJOR) {
+      const uint32_t s_from = ring + slot * kStep + 1024 + g * 4;
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s0) : "r"(s_from));
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s1) : "r"(s_from + 32));
+    }
+    float c[NT][4];
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      uint32_t a[8];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const uint4& v = h ? v1 : v0;
+        const uint32_t word = q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) a[2 * k + h] = codes_pair<T>(word >> (4 * k), bias);
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        const uint4 b = ptx::lds128(((b_at[nt] + b_off) ^ ((q & 1) * 64)) + (q >> 1) * 128);
+        if (q == 0) mma16<T, false>(c[nt], a[0], a[1], a[2], a[3], b.x, b.y);
+        else mma16<T, true>(c[nt], a[0], a[1], a[2], a[3], b.x, b.y);
+        mma16<T, true>(c[nt], a[4], a[5], a[6], a[7], b.z, b.w);
+      }
+    }
+    __syncwarp();                                                   // the slot has been read
+    if (i + DEPTH < total) fetch(slot);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (++slot == DEPTH) slot = 0;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) f[nt][i] = 0.f;
-    uint32_t b_off = first * M * 256;
-    int u = 0, tile = wn;
-    int slot = 0;
-    {
-      for (int i = 0; i < total; ++i) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(DEPTH - 1) : "memory");
-        __syncwarp();
-        {
-          const uint32_t from = ring_lane + slot * kStep;
-          const uint4 v0 = ptx::lds128(from), v1 = ptx::lds128(from + 512);
-          float s0 = 1.0f, s1 = 1.0f;
-          if constexpr (!ROWMAJOR) {
-            const uint32_t s_from = ring + slot * kStep + 1024 + g * 4;
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s0) : "r"(s_from));
-            asm volatile("ld.shared.f32 %0, [%1];" : "=f"(s1) : "r"(s_from + 32));
-          }
-          float c[NT][4];
+      for (int j = 0; j < 4; ++j) f[nt][j] = fmaf(c[nt][j], j >> 1 ? s1 : s0, f[nt][j]);
+    b_off += M * 256;
+    if (++u == mine) {                                              // the tile's sums over this warp's units
+      float* to = part + (tile * k_warps + wk) * M * 16;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            uint32_t a[8];
+      for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-              const uint4& v = h ? v1 : v0;
-              const uint32_t word = q == 0 ? v.x : q == 1 ? v.y : q == 2 ? v.z : v.w;
-              if constexpr (PLAIN) {
-#pragma unroll
-                for (int k = 0; k < 4; ++k) a[2 * k + h] = codes_pair<T>(word >> (4 * k), bias);
-              } else {
-                a[h] = mask_flip<0x000F000Fu>(word, flip_lo);
-                a[2 + h] = mask_flip<0x00F000F0u>(word, flip_hi);
-                a[4 + h] = mask_flip<0x000F000Fu>(word >> 8, flip_lo);
-                a[6 + h] = mask_flip<0x00F000F0u>(word >> 8, flip_hi);
-              }
-            }
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              const uint4 b = ptx::lds128(((b_at[nt] + b_off) ^ ((q & 1) * 64)) + (q >> 1) * 128);
-              using A = std::conditional_t<PLAIN, T, __half>;
-              if (q == 0) mma16<A, false>(c[nt], a[0], a[1], a[2], a[3], b.x, b.y);
-              else mma16<A, true>(c[nt], a[0], a[1], a[2], a[3], b.x, b.y);
-              mma16<A, true>(c[nt], a[4], a[5], a[6], a[7], b.z, b.w);
-            }
-          }
-          __syncwarp();                                                   // the slot has been read
-          if (i + DEPTH < total) fetch(slot);
-          asm volatile("cp.async.commit_group;" ::: "memory");
-          if (++slot == DEPTH) slot = 0;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            float4 k = make_float4(1.f, 0.f, 1.f, 0.f);
-            if constexpr (!PLAIN) k = *reinterpret_cast<const float4*>(ab + ((first + u) * NT + nt) * 8 + 2 * t);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              const float s = PLAIN ? c[nt][j] : fmaf(c[nt][j], j & 1 ? k.z : k.x, j & 1 ? -k.w : -k.y);
-              f[nt][j] = fmaf(s, j >> 1 ? s1 : s0, f[nt][j]);
-            }
-          }
-          b_off += M * 256;
-          if (++u == mine) {                                              // the tile's sums over this warp's units
-            float* to = part + (tile * k_warps + wk) * M * 16;
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                const int m = 8 * nt + 2 * t + (j & 1);
-                if (m < M) to[m * 16 + g + 8 * (j >> 1)] = f[nt][j];
-                f[nt][j] = 0.f;
-              }
-            u = 0;
-            b_off = first * M * 256;
-            tile += p.tile_warps;
-          }
+        for (int j = 0; j < 4; ++j) {
+          const int m = 8 * nt + 2 * t + (j & 1);
+          if (m < M) to[m * 16 + g + 8 * (j >> 1)] = f[nt][j];
+          f[nt][j] = 0.f;
         }
-      }
+      u = 0;
+      b_off = first * M * 256;
+      tile += p.tile_warps;
     }
-  };
-  if constexpr (NT == 1) {
-    if (!plain) walk(std::false_type{});
   }
-  if (plain) walk(std::true_type{});
   __syncthreads();
 
   // the warps' sums in ascending order (those that have units), then the ranks'
