@@ -263,6 +263,7 @@ class Qwen3Prefill(nn.Module):
         """One token, a chain or a tree of drafts of every sequence: ids [B, T] -> final hidden states [B, T, hidden].  In a tree node t sees
         the nodes j with ``tree_mask[b, t, j]`` (bool, itself and its ancestors) and stands that many positions behind the cache.
         ``cache.commit`` keeps the accepted ones; until then the cache is as it was, and the next ``step`` forgets them."""
+        cache.pending, made = [], []     # a step that raises half-way leaves nothing to commit
         B, T = ids.shape
         freqs = cache.freqs
         if tree_mask is None:
@@ -271,11 +272,12 @@ class Qwen3Prefill(nn.Module):
             depth = tree_mask.sum(-1) - 1
         positions = (cache.lengths[:, None] + depth).flatten()
         x = self.embed(ids)
-        cache.pending = []
         for layer, blk in enumerate(self.blocks):
             def attend(q, k, v, layer=layer):
-                cache.pending.append((k, v))
+                made.append((k, v))
                 return ops.tree_attention(q, k, v, cache.k[layer], cache.v[layer], cache.block_table, cache.lengths, tree_mask=tree_mask)
 
             x = blk.step(x, positions, freqs, attend)
-        return self.norm(x)
+        x = self.norm(x)
+        cache.pending = made
+        return x
