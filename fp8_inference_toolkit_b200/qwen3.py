@@ -242,7 +242,7 @@ class Qwen3Prefill(nn.Module):
     def prefill(self, ids: torch.Tensor, cache: DecodeCache, counts: torch.Tensor | None = None) -> torch.Tensor:
         """As ``forward`` for prompts [B, S] of which ``counts[b]`` tokens count (int32; all without), whose keys and values go into the empty
         sequences of ``cache``."""
-        cfg = self.cfg
+        cache.pending = []     # a step before the prompt is none behind it
         B, S = ids.shape
         freqs = cache.freqs
         positions = torch.arange(S, device=ids.device).repeat(B)

@@ -66,3 +66,19 @@ def test_a_step_that_raised_cannot_be_committed(decode, layer, when):
     model.step(IDS, cache)
     cache.commit()
     assert len(appended) == 3 and cache.lengths.tolist() == [3, 3]
+
+
+@pytest.mark.parametrize("fails", [None, "before"])
+def test_prefill_forgets_the_step_before_it(decode, fails):
+    make, appended = decode
+    model, cache = make(_Layer(), _Layer())
+    model.step(IDS, cache)
+    model.blocks[1].fails = fails
+    if fails:
+        with pytest.raises(RuntimeError, match="failed"):
+            model.prefill(IDS, cache)
+    else:
+        model.prefill(IDS, cache)
+    with pytest.raises(RuntimeError, match="no step"):
+        cache.commit()
+    assert not appended
