@@ -208,14 +208,40 @@ class DecodeCache:
     def append(self, layer: int, k, v, counts=None, select=None) -> None:
         ops.kv_cache_append_(self.k[layer], self.v[layer], k, v, self.block_table, self.lengths, select=select, counts=counts)
 
+    def accepted(self, tokens: int, counts: torch.Tensor | None = None, select: torch.Tensor | None = None) -> torch.Tensor:
+        """[batch] int32: how many of `tokens` new rows each sequence takes, all of ``counts[b]`` (all rows without), or -1 where it can take them
+        not at all: a count or an index of ``select`` out of range, no room, or a page that the table does not name.  An append with -1 writes
+        nothing and is raised by ``ops.check_status``; nothing here waits for the device."""
+        B, width = self.block_table.shape
+        dev = self.lengths.device
+        if counts is None:
+            counts = torch.full_like(self.lengths, tokens)
+        elif counts.dtype != torch.int32 or counts.shape != (B,) or counts.device != dev:
+            raise RuntimeError("counts must be int32 [batch], on the cache's device")
+        row = torch.arange(tokens, device=dev)
+        at = self.lengths.long()[:, None] + row
+        page_size = self.k[0].shape[1]
+        fits = (at >= 0) & (at < width * page_size)
+        if width:
+            page = self.block_table.gather(1, (at // page_size).clamp(0, width - 1))
+            fits &= (page >= 0) & (page < self.k[0].shape[0])
+        if select is not None:
+            if select.dtype != torch.int32 or select.dim() != 2 or select.shape[0] != B or select.shape[1] < tokens or select.device != dev:
+                raise RuntimeError("select must be int32 [batch, new rows], on the cache's device")
+            fits &= (select[:, :tokens] >= 0) & (select[:, :tokens] < tokens)
+        ok = (fits | (row >= counts[:, None])).all(1) & (counts >= 0) & (counts <= tokens)
+        return torch.where(ok, counts, -1)
+
     def commit(self, counts: torch.Tensor | None = None, select: torch.Tensor | None = None) -> None:
         """Keeps ``counts[b]`` tokens of the last step (all without): its first ones, or rows ``select[b, :counts[b]]``, the accepted path of a
-        tree.  int32; nothing waits for the device."""
+        tree.  int32; nothing waits for the device.  A sequence that cannot take its tokens (``accepted``) keeps its length and its
+        cache, which ``ops.check_status`` raises."""
         if not self.pending:
             raise RuntimeError("commit: there is no step to keep tokens of")
+        counts = self.accepted(self.pending[0][0].shape[1], counts, select)
         for layer, (k, v) in enumerate(self.pending):
             self.append(layer, k, v, counts, select)
-        self.lengths += self.pending[0][0].shape[1] if counts is None else counts
+        self.lengths += counts.clamp(min=0)
         self.pending = []
 
 
@@ -241,11 +267,12 @@ class Qwen3Prefill(nn.Module):
     @torch.no_grad()
     def prefill(self, ids: torch.Tensor, cache: DecodeCache, counts: torch.Tensor | None = None) -> torch.Tensor:
         """As ``forward`` for prompts [B, S] of which ``counts[b]`` tokens count (int32; all without), whose keys and values go into the empty
-        sequences of ``cache``."""
+        sequences of ``cache``.  One that cannot take them (``DecodeCache.accepted``) stays as it was, which ``ops.check_status`` raises."""
         cache.pending = []     # a step before the prompt is none behind it
         B, S = ids.shape
         freqs = cache.freqs
         positions = torch.arange(S, device=ids.device).repeat(B)
+        counts = cache.accepted(S, counts)
         x = self.embed(ids)
         for layer, blk in enumerate(self.blocks):
             def attend(blk, qkv, layer=layer):
@@ -255,7 +282,7 @@ class Qwen3Prefill(nn.Module):
                 return a.transpose(1, 2).reshape(B, S, -1)
 
             x = blk(x, None, None, attend)
-        cache.lengths += S if counts is None else counts
+        cache.lengths += counts.clamp(min=0)
         return self.norm(x)
 
     @torch.no_grad()

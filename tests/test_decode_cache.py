@@ -82,3 +82,68 @@ def test_prefill_forgets_the_step_before_it(decode, fails):
     with pytest.raises(RuntimeError, match="no step"):
         cache.commit()
     assert not appended
+
+
+def _cache(make, lengths, tokens=12):
+    model, cache = make(_Layer(), _Layer(), batch=len(lengths), tokens=tokens)
+    cache.lengths.copy_(torch.tensor(lengths))
+    return model, cache
+
+
+@pytest.mark.parametrize("lengths,counts,taken", [
+    ([0, 5], None, [3, 3]), ([9, 10], None, [3, -1]), ([12, 11], [0, 1], [0, 1]), ([12, 11], [1, 2], [-1, -1]), ([0, 0], [4, -1], [-1, -1]),
+    ([-1, 13], [1, 0], [-1, 0]), ([-2, 2 ** 31 - 1], [3, 3], [-1, -1]),
+])
+def test_lengths_count_what_was_appended(decode, lengths, counts, taken):
+    """Full sequences, counts out of range and lengths out of range: such a sequence takes nothing and is reported by its count of -1."""
+    make, appended = decode
+    model, cache = _cache(make, lengths)
+    model.step(IDS, cache)
+    cache.commit(None if counts is None else torch.tensor(counts, dtype=torch.int32))
+    assert [c.tolist() for _, _, c in appended] == [taken] * 2
+    assert cache.lengths.tolist() == [n + max(0, t) for n, t in zip(lengths, taken)] and cache.lengths.dtype == torch.int32
+
+
+@pytest.mark.parametrize("counts,taken,tokens", [(None, [3, 3], 12), ([3, 0], [3, 0], 12), ([4, 2], [0, 2], 12), ([-1, 1], [0, 1], 12), (None, [0, 0], 0)])
+def test_lengths_count_what_a_prompt_appended(decode, counts, taken, tokens):
+    make, _ = decode
+    model, cache = _cache(make, [0, 0], tokens)
+    model.prefill(IDS, cache, None if counts is None else torch.tensor(counts, dtype=torch.int32))
+    assert cache.lengths.tolist() == taken
+
+
+def test_pages_and_rows_that_do_not_exist(decode):
+    make, appended = decode
+    model, cache = _cache(make, [4, 3])
+    cache.block_table[0, 1], cache.block_table[1, 2] = -1, 6       # 6 pages there are; the second page of sequence 1 is the last it needs
+    model.step(IDS, cache)
+    cache.commit()
+    assert appended[0][2].tolist() == [-1, 3] and cache.lengths.tolist() == [4, 6]
+    model.step(IDS, cache)
+    cache.commit(torch.tensor([0, 2], dtype=torch.int32), torch.tensor([[9, 9, 9], [0, 2, 9]], dtype=torch.int32))
+    assert appended[-1][2].tolist() == [0, 2] and cache.lengths.tolist() == [4, 8]
+    cache.block_table[1, 2] = 5
+    model.step(IDS, cache)
+    cache.commit(torch.tensor([0, 2], dtype=torch.int32), torch.tensor([[0, 0, 0], [0, 3, 0]], dtype=torch.int32))
+    assert appended[-1][2].tolist() == [0, -1] and cache.lengths.tolist() == [4, 8]
+
+
+def test_a_cache_without_room(decode):
+    make, appended = decode
+    model, cache = _cache(make, [0, 0], tokens=0)
+    model.step(IDS, cache)
+    cache.commit()
+    assert appended[0][2].tolist() == [-1, -1] and cache.lengths.tolist() == [0, 0]
+
+
+def test_counts_and_rows_of_another_kind_are_refused(decode):
+    make, appended = decode
+    model, cache = _cache(make, [0, 0])
+    model.step(IDS, cache)
+    for counts, select in [(torch.ones(2), None), (torch.ones(1, dtype=torch.int32), None), (None, torch.zeros(2, 3)),
+                           (None, torch.zeros(2, 2, dtype=torch.int32)), (None, torch.zeros(1, 3, dtype=torch.int32))]:
+        with pytest.raises(RuntimeError, match="counts must be" if counts is not None else "select must be"):
+            cache.commit(counts, select)
+    assert not appended and cache.lengths.tolist() == [0, 0]
+    cache.commit()
+    assert cache.lengths.tolist() == [3, 3]
