@@ -208,10 +208,11 @@ class DecodeCache:
     def append(self, layer: int, k, v, counts=None, select=None) -> None:
         ops.kv_cache_append_(self.k[layer], self.v[layer], k, v, self.block_table, self.lengths, select=select, counts=counts)
 
-    def accepted(self, tokens: int, counts: torch.Tensor | None = None, select: torch.Tensor | None = None) -> torch.Tensor:
+    def accepted(self, tokens: int, counts: torch.Tensor | None = None, select: torch.Tensor | None = None, prompt: bool = False) -> torch.Tensor:
         """[batch] int32: how many of `tokens` new rows each sequence takes, all of ``counts[b]`` (all rows without), or -1 where it can take them
-        not at all: a count or an index of ``select`` out of range, no room, or a page that the table does not name.  An append with -1 writes
-        nothing and is raised by ``ops.check_status``; nothing here waits for the device."""
+        not at all: a count or an index of ``select`` out of range, no room, a page that the table does not name, or (``prompt``) tokens for a
+        sequence that is not empty.  An append with -1 writes nothing and is raised by ``ops.check_status``; nothing here waits
+        for the device."""
         B, width = self.block_table.shape
         dev = self.lengths.device
         if counts is None:
@@ -230,6 +231,8 @@ class DecodeCache:
                 raise RuntimeError("select must be int32 [batch, new rows], on the cache's device")
             fits &= (select[:, :tokens] >= 0) & (select[:, :tokens] < tokens)
         ok = (fits | (row >= counts[:, None])).all(1) & (counts >= 0) & (counts <= tokens)
+        if prompt:
+            ok &= (self.lengths == 0) | (counts == 0)
         return torch.where(ok, counts, -1)
 
     def commit(self, counts: torch.Tensor | None = None, select: torch.Tensor | None = None) -> None:
@@ -267,12 +270,13 @@ class Qwen3Prefill(nn.Module):
     @torch.no_grad()
     def prefill(self, ids: torch.Tensor, cache: DecodeCache, counts: torch.Tensor | None = None) -> torch.Tensor:
         """As ``forward`` for prompts [B, S] of which ``counts[b]`` tokens count (int32; all without), whose keys and values go into the empty
-        sequences of ``cache``.  One that cannot take them (``DecodeCache.accepted``) stays as it was, which ``ops.check_status`` raises."""
+        sequences of ``cache``; a sequence without such tokens is left as it is.  One that cannot take its tokens (``DecodeCache.accepted``),
+        because it is not empty for instance, stays as it was too, which ``ops.check_status`` raises."""
         cache.pending = []     # a step before the prompt is none behind it
         B, S = ids.shape
         freqs = cache.freqs
         positions = torch.arange(S, device=ids.device).repeat(B)
-        counts = cache.accepted(S, counts)
+        counts = cache.accepted(S, counts, prompt=True)
         x = self.embed(ids)
         for layer, blk in enumerate(self.blocks):
             def attend(blk, qkv, layer=layer):

@@ -147,3 +147,23 @@ def test_counts_and_rows_of_another_kind_are_refused(decode):
     assert not appended and cache.lengths.tolist() == [0, 0]
     cache.commit()
     assert cache.lengths.tolist() == [3, 3]
+
+
+def test_prompts_go_into_empty_sequences(decode, monkeypatch):
+    """A prompt's positions begin at 0 and it sees itself only: a sequence that holds tokens takes none; without tokens it is left alone."""
+    make, _ = decode
+    model, cache = _cache(make, [4, 0])
+    model.prefill(IDS, cache)
+    assert cache.lengths.tolist() == [4, 3]
+    model.prefill(IDS, cache, torch.tensor([0, 1], dtype=torch.int32))
+    assert cache.lengths.tolist() == [4, 3]
+    asked = []
+    monkeypatch.setattr(type(cache), "append", lambda self, layer, k, v, counts=None, select=None: asked.append(counts.tolist()))
+    monkeypatch.setattr(_Layer, "forward", lambda self, x, cos, sin, attend: attend(self, x))
+    monkeypatch.setattr(_Layer, "_turned_heads", lambda self, qkv, positions, freqs: (qkv[:, None],) * 3, raising=False)
+    cache.lengths.copy_(torch.tensor([0, 1]))
+    model.prefill(IDS, cache, torch.tensor([2, 1], dtype=torch.int32))
+    assert asked and set(map(tuple, asked)) == {(2, -1)} and cache.lengths.tolist() == [2, 1]
+    asked.clear()
+    model.prefill(IDS, cache, torch.tensor([0, 0], dtype=torch.int32))
+    assert set(map(tuple, asked)) == {(0, 0)} and cache.lengths.tolist() == [2, 1]

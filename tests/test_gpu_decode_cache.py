@@ -43,3 +43,21 @@ def test_a_sequence_that_cannot_take_its_tokens(case):
                     at = before[b] + i
                     want[int(cache.block_table[b, at // 16]), at % 16] = value[b, i if select is None else int(select[b, i])]
             assert torch.equal(cached, want)
+
+
+def test_a_prompt_for_a_sequence_that_is_not_empty():
+    """It takes none of its tokens and says so; the others take theirs, and one without tokens is no fault."""
+    from fp8_inference_toolkit_b200 import ops
+    from fp8_inference_toolkit_b200.qwen3 import DecodeCache, Qwen3Config, Qwen3Prefill
+
+    cfg = Qwen3Config(hidden=512, layers=1, q_heads=4, kv_heads=2, head_dim=128, inter=512, vocab=64)
+    model, cache = Qwen3Prefill(cfg), DecodeCache(cfg, 3, 32, page_size=16)
+    ids = torch.arange(24, device="cuda").view(3, 8)
+    model.prefill(ids, cache, torch.tensor([8, 0, 5], dtype=torch.int32, device="cuda"))
+    ops.check_status()
+    held = cache.k[0].clone()
+    model.prefill(ids.flip(1), cache, torch.tensor([0, 8, 8], dtype=torch.int32, device="cuda"))
+    assert cache.lengths.tolist() == [8, 8, 5]
+    assert torch.equal(cache.k[0][:2], held[:2]) and torch.equal(cache.k[0][4:], held[4:]) and cache.k[0][2, :8].any()
+    with pytest.raises(RuntimeError, match="out of range"):
+        ops.check_status()
