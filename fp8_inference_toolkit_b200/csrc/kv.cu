@@ -973,7 +973,7 @@ extern "C" int i4tc_tree_attention(const i4tc_tree_attention_args* a, int device
                    a->table_width >= 0 && a->table_width < (1ll << 31), I4TC_EINVAL, "bad size");
   I4TC_REQUIRE(isfinite(a->scale) && fabs(a->scale) < 1e30, I4TC_EINVAL, "the scale must be finite");
   I4TC_REQUIRE(a->q && a->k && a->v && a->lengths && a->out, I4TC_EINVAL, "null pointer");
-  I4TC_REQUIRE(a->table_width == 0 || a->pages == 0 || (a->k_cache && a->v_cache && a->block_table), I4TC_EINVAL, "null pointer");
+  I4TC_REQUIRE(a->table_width == 0 || (a->block_table && (a->pages == 0 || (a->k_cache && a->v_cache))), I4TC_EINVAL, "null pointer");
   I4TC_REQUIRE(aligned_to(a->k, 16) && aligned_to(a->v, 16) && aligned_to(a->k_cache, 16) && aligned_to(a->v_cache, 16) &&
                    aligned_to(a->q, 4) && aligned_to(a->out, 16) && aligned_to(a->scratch, 16) && a->q_batch % 2 == 0 && a->q_token % 2 == 0 &&
                    a->q_head % 2 == 0 && (a->new_batch | a->new_token | a->new_head | a->page_stride | a->slot_stride | a->head_stride) % 8 == 0,
@@ -1022,7 +1022,7 @@ extern "C" int i4tc_kv_append(const i4tc_kv_append_args* a, int device, void* st
                    a->pages < (1ll << 31) && a->page_size > 0 && a->page_size < (1ll << 31) && a->table_width >= 0 && a->table_width < (1ll << 31),
                I4TC_EINVAL, "bad size");
   I4TC_REQUIRE(a->k && a->v && a->lengths, I4TC_EINVAL, "null pointer");
-  I4TC_REQUIRE(a->table_width == 0 || a->pages == 0 || (a->k_cache && a->v_cache && a->block_table), I4TC_EINVAL, "null pointer");
+  I4TC_REQUIRE(a->table_width == 0 || (a->block_table && (a->pages == 0 || (a->k_cache && a->v_cache))), I4TC_EINVAL, "null pointer");
   const DeviceInfo* info;
   if (int rc = device_info(device, &info)) return rc;
   AppendParams p = {};
