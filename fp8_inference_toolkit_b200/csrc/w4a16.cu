@@ -16,7 +16,7 @@
 // Codes become operands of the tokens' type by masking and a subtraction: a nibble with its top bit flipped, in the low bits of the
 // number 128 (bf16) or 1024 (fp16), is that number + 8 + code, and the difference is exact.  So are the products, and the fp32 sums hold
 // nothing but the formula's terms: where a code is zero, the token's number has no part, however large.  (Leaving the +8 in and taking 8
-// times the tokens' sum off the result saves the subtraction, 14.9 us instead of 16.4 for one gated token, but a number
+// times the tokens' sum off the result saves the subtraction, 1.5 us of 16.4 for one gated token, but a number
 // 2^20 times as large as the others then costs their sums 20 bits wherever its code is zero.)
 //
 // The k order inside an instruction is free as long as both operands agree: a word's nibbles come out as pairs (i, i + 4), and the
@@ -26,8 +26,8 @@
 // laying them out in every block costs more than adding up; its partial sums are added in ascending order through distributed
 // shared memory: no workspace, no second launch, and the same bits in every run.
 //
-// Measured (device time, weights from HBM, bf16, per-group scales): [1, 4096] x [6144, 4096] 6.5 us, [16, 12288] x [4096, 12288]
-// 14.4, gated [1, 4096] x [24576, 4096] 16.4 (3.3 TB/s), [16, ...] 21.7, [32, ...] 37.3.
+// Measured (device time, weights from HBM, bf16, per-group scales): [1, 4096] x [6144, 4096] 5.9 us, [16, 12288] x [4096, 12288]
+// 14.4, gated [1, 4096] x [24576, 4096] 16.0 (3.3 TB/s), [16, ...] 20.9, [32, ...] 37.3.
 #include "common.cuh"
 #include "ptx.cuh"
 #include <type_traits>
@@ -497,13 +497,23 @@ extern "C" int i4tc_w4a16_linear(const i4tc_w4a16_args* a, int device, void* str
       if (w4a16_smem(tokens, small, each, block_tiles, k_warps) > kMostSmem) continue;
       const int64_t waves = ((int64_t)gx * chunks + at_once[i] - 1) / at_once[i];
       const int warp_steps = (block_tiles + tw - 1) / tw * steps;
-      // Microseconds: a step of a block costs its instructions, or a warp's steps their latency; the tokens' rows are laid out by
-      // every block; sums are added per warp that splits K, and between the ranks of a cluster.
-      const double issue = (0.8 * block_tiles * each + 0.2 * kWarps * warp_steps) * (nt == 1 ? 0.033 : nt == 2 ? 0.05 : nt == 3 ? 0.074 : 0.098);
-      const double latency = warp_steps * 0.35;
-      const double layout = each * tokens * (nt == 1 ? 0.011 : 0.006);
-      const double sums = (double)block_tiles * tokens * 16 * (k_warps - 1) * 0.0005;
-      const double cost = waves * ((issue > latency ? issue : latency) + layout + sums) + (ranks > 1 ? 0.7 : 0.0);
+      // Microseconds.  A warp scheduler (it has every fourth warp) issues its warps' steps one after the other, or a warp's steps take their
+      // latency; before that the tokens' rows are laid out by every block, after it threads add what the warps that split K have,
+      // and ranks what the others have.  What it is for: 1 x 4096 x 4096 takes 4.7 us in blocks of two tile warps and 6.1 in
+      // clusters of four, gated 8 x 4096 x 2 * 12288 17.1 with sixteen tile warps and 29.7 with sixteen that split K.  The constants are
+      // fitted to 7 thousand timings (K 512 to 12288, 64 to 12288 columns, 1 to 32 tokens, all ways to split): the choice is 0.7 %
+      // slower than the fastest way on average, 15 % at most; 1.4 % and 22 % at sizes that they were not fitted to.
+      int issued = (block_tiles + 3) / 4 * each;
+      if (tw < 4) {
+        issued = 0;
+        for (int k = 0; k < k_warps; k += 4 / tw) issued += each > (k + 1) * steps ? steps : each > k * steps ? each - k * steps : 0;
+        issued *= (block_tiles + tw - 1) / tw;
+      }
+      const double issue = issued * (nt == 1 ? 0.143 : nt == 2 ? 0.2 : nt == 3 ? 0.278 : 0.333);
+      const double latency = warp_steps * (0.3 + 0.01 * nt);
+      const int rounds = (block_tiles * tokens * cols + kThreads - 1) / kThreads;
+      const double sums = (rounds + ranks - 1) / ranks * ((each + steps - 1) / steps) * 0.063;
+      const double cost = waves * (0.7 + (issue > latency ? issue : latency) + each * tokens * 0.0034 + sums) + (ranks > 1 ? 1.5 + 0.07 * i : 0.0);
       if (grid_x == 0 || cost < best) {
         best = cost;
         grid_x = gx;
