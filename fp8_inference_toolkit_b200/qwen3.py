@@ -102,8 +102,8 @@ class Block(nn.Module):
         self.ln2 = RMSNorm(cfg.hidden, cfg.eps, device)
         self.q_norm = RMSNorm(cfg.head_dim, cfg.eps, device)
         self.k_norm = RMSNorm(cfg.head_dim, cfg.eps, device)
-        # fold the quantisers into RMSNorm / SwiGLU (per-group scales only; the per-channel ops keep the plain path)
-        self.fused = fused and not per_channel
+        # fold the quantisers into RMSNorm / SwiGLU (per-group scales only; the per-channel ops and 16-bit activations keep the plain path)
+        self.fused = fused and not per_channel and self.qkv.method.act_bits == 4
 
     @staticmethod
     def _lin(k, n, device, per_channel, gen):
