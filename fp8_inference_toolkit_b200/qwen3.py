@@ -89,6 +89,11 @@ def apply_rope(x, cos, sin):
     return torch.cat([x1 * c - x2 * s, x2 * c + x1 * s], dim=-1)
 
 
+def _bare(*linears) -> bool:
+    """Whether these linears are their product and nothing else: no smoothing factors for the inputs, no bias."""
+    return all(lin.smooth_scale is None and lin.bias is None for lin in linears)
+
+
 class Block(nn.Module):
     def __init__(self, cfg: Qwen3Config, device, per_channel: bool, gen: torch.Generator, fused: bool = True):
         super().__init__()
@@ -117,7 +122,7 @@ class Block(nn.Module):
     def forward(self, x, cos, sin, attend=None):
         cfg = self.cfg
         B, S, _ = x.shape
-        if self.fused:
+        if self.fused and _bare(self.qkv, self.gate_up, self.down):
             return self._forward_fused(x, cos, sin, attend)
         qkv = self.qkv(self.ln1(x))
         if attend is not None:
@@ -147,13 +152,20 @@ class Block(nn.Module):
         B, T, H = x.shape
 
         def linear(lin, y):
-            return ops.w4a16_linear(y, lin.weight_int4, lin.weight_scale, lin.out_features, lin.method.per_channel)
+            if lin.smooth_scale is not None:
+                y = y / lin.smooth_scale.to(y.dtype)
+            y = ops.w4a16_linear(y, lin.weight_int4, lin.weight_scale, lin.out_features, lin.method.per_channel)
+            return y if lin.bias is None else y + lin.bias
 
         heads = self._turned_heads(linear(self.qkv, self.ln1(x).view(B * T, H)), positions, freqs)
         a = attend(*(t.unflatten(0, (B, T)) for t in heads))
         x = x + linear(self.o, a.view(B * T, -1)).view(B, T, H)
-        up = ops.w4a16_gated_linear(self.ln2(x).view(B * T, H), self.gate_up.weight_int4, self.gate_up.weight_scale, cfg.inter,
-                                    self.gate_up.method.per_channel)
+        y = self.ln2(x).view(B * T, H)
+        if _bare(self.gate_up):
+            up = ops.w4a16_gated_linear(y, self.gate_up.weight_int4, self.gate_up.weight_scale, cfg.inter, self.gate_up.method.per_channel)
+        else:
+            gate, up = linear(self.gate_up, y).split(cfg.inter, -1)
+            up = F.silu(gate) * up
         return x + linear(self.down, up).view(B, T, H)
 
     def _attention(self, qkv, B, S, cos, sin):
