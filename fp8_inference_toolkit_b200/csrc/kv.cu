@@ -878,18 +878,29 @@ int padded_dim(int64_t D) { return D <= 64 ? 64 : 128; }
 struct AttendPlan {
   int ranks, parts;
 };
-AttendPlan attend_plan(int sm_count, int64_t batch, int64_t lines, int64_t most_length, int64_t tokens) {
+AttendPlan attend_plan(int sm_count, int64_t batch, int64_t kv_heads, int64_t rows, int64_t D, int64_t most_length, int64_t tokens) {
+  const int warps = row_warps(rows);
+  const int64_t row_tiles = (rows + 16 * warps - 1) / (16 * warps), lines = kv_heads * row_tiles;
   const int64_t tiles = (most_length + tokens + kTile - 1) / kTile, slots = (int64_t)sm_count * 2;
   const int64_t most = slots / lines < 1 ? 1 : slots / lines;
   AttendPlan plan = {0, (int)(batch * tiles < most ? batch * tiles : most)};
-  // Microseconds, by the room in the table: a block's way to its first tile and its end, its tiles, and for parts the second kernel.
-  double best = 4.0 + 5.0 + 1.1 * (double)((batch * tiles + plan.parts - 1) / plan.parts) * ((plan.parts * lines + slots - 1) / slots);
-  for (int ranks = 1; ranks <= 8; ranks *= 2) {
-    const int64_t waves = (batch * lines * ranks + slots - 1) / slots;
-    const double cost = waves * (4.0 + 1.1 * (double)((tiles + ranks - 1) / ranks)) + (ranks > 1 ? 1.5 : 0.0);
+  // Microseconds, by the room in the table, from 344 sizes timed all five ways (lengths from an eighth of the room to all of it): a block's way
+  // to its first tile and its end, its tiles, a cluster's sums; for parts the second kernel (9.4 with everything, and 2.5 of the
+  // 5 that a call of it costs the host more).  What it is for, 8 key heads of 128 and 4 query heads each, clusters of 1, 2, 4, 8 | parts: one token
+  // over 32000 564 us, 288, 149, 79 | 34; 64 trees of four over up to 256 24, 46, 80, 165 | 33.  The choice is 2.7 % slower on
+  // the device than the fastest way on average and 34 % at most; 3.4 % and 46 % at 378 sizes that it was not fitted to.
+  const double tile = (warps == 1 ? 1.15 : warps == 2 ? 1.43 : 1.88) * (padded_dim(D) == 64 ? 0.64 : 1.0);
+  const int64_t line_rows = rows < 16 * warps ? rows : 16 * warps;
+  double best = 9.4 + 2.5 + 0.97 * tile * (double)((batch * tiles + plan.parts - 1) / plan.parts * ((plan.parts * lines + slots - 1) / slots)) +
+                0.2e-3 * (double)(batch * lines * line_rows);
+  for (int i = 0; i < 4; ++i) {
+    const int64_t ranks = 1 << i;
+    const double load = (double)(batch * lines * ranks) / ((double)slots * (i < 2 ? 1.0 : i == 2 ? 0.89 : 0.81));   // clusters do not cross a GPC
+    const double waves = load <= 1.0 ? 1.0 : 0.87 * load + 0.13 * ceil(load);
+    const double cost = 0.4 + waves * (4.6 + tile * (double)((tiles + ranks - 1) / ranks)) + (i > 0 ? 3.5 + 0.36 * i : 0.0);
     if (cost < best && batch * lines * ranks < (1ll << 30)) {
       best = cost;
-      plan.ranks = ranks;
+      plan.ranks = (int)ranks;
     }
   }
   return plan;
@@ -956,7 +967,7 @@ extern "C" int64_t i4tc_tree_attention_scratch_bytes(int64_t batch, int64_t toke
   const int64_t rows = tokens * (heads / kv_heads);
   const int tile_rows = 16 * row_warps(rows);
   const int64_t lines = kv_heads * ((rows + tile_rows - 1) / tile_rows);
-  const AttendPlan plan = attend_plan(info->sm_count, batch, lines, most_length, tokens);
+  const AttendPlan plan = attend_plan(info->sm_count, batch, kv_heads, rows, D, most_length, tokens);
   return plan.ranks ? 0 : plan.parts * lines * 2 * (int64_t)slot_floats(tile_rows, padded_dim(D)) * 4;
 }
 
@@ -998,7 +1009,7 @@ extern "C" int i4tc_tree_attention(const i4tc_tree_attention_args* a, int device
   const int64_t most_length = a->table_width * a->page_size;
   I4TC_REQUIRE(most_length < (1ll << 31) - 2 * kTile && a->batch * ((most_length + a->tokens) / kTile + 1) < (1ll << 31) && a->batch * p.lines < (1ll << 24),
                I4TC_EUNSUPPORTED, "the table has room for too many tokens");
-  const AttendPlan plan = attend_plan(info->sm_count, a->batch, p.lines, most_length, a->tokens);
+  const AttendPlan plan = attend_plan(info->sm_count, a->batch, p.kv_heads, rows, p.D, most_length, a->tokens);
   p.parts = plan.parts;
   p.ranks = plan.ranks;
   I4TC_REQUIRE(p.ranks || a->scratch != nullptr, I4TC_EINVAL, "null pointer");
