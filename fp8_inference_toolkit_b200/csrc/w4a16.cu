@@ -36,7 +36,7 @@ namespace i4tc {
 
 namespace {
 
-constexpr int kWarps = 16, kThreads = kWarps * 32;
+constexpr int kLogWarps = 4, kWarps = 1 << kLogWarps, kThreads = kWarps * 32;
 constexpr int kMostTokens = 32;                     // of a launch's grid row; more tokens read the weights again
 constexpr size_t kMostSmem = 224 * 1024;
 constexpr int kStep = 16 * 64 + 16 * 4;             // bytes of a step: sixteen rows of 128 codes, and their scales
@@ -484,19 +484,19 @@ extern "C" int i4tc_w4a16_linear(const i4tc_w4a16_args* a, int device, void* str
     if (ranks > p.units || at_once[i] < 1) continue;
     const int each = (p.units + ranks - 1) / ranks;
     if ((ranks - 1) * each >= p.units) continue;
-    for (int tw = 1; tw <= kWarps; tw *= 2) {
-      const int k_warps = kWarps / tw, steps = (each + k_warps - 1) / k_warps;
-      int gx = at_once[i] > p.tiles ? p.tiles : at_once[i];
+    const int most_x = at_once[i] > p.tiles ? p.tiles : at_once[i], most_tiles = (p.tiles + most_x - 1) / most_x;
+    for (int j = 0; 1 << j <= kWarps; ++j) {   // (shifts: the way is chosen in every call, which waits for the host where it is short)
+      const int tw = 1 << j, k_warps = kWarps >> j, steps = (each + k_warps - 1) >> (kLogWarps - j);
       // partial sums of all of a block's tiles have to fit: else more blocks, in waves
-      int block_tiles = (p.tiles + gx - 1) / gx;
+      int gx = most_x, block_tiles = most_tiles;
       while (block_tiles > 1 && w4a16_smem(tokens, small, each, block_tiles, k_warps) > kMostSmem) {
         gx *= 2;
         gx = gx > p.tiles ? p.tiles : gx;
         block_tiles = (p.tiles + gx - 1) / gx;
       }
       if (w4a16_smem(tokens, small, each, block_tiles, k_warps) > kMostSmem) continue;
-      const int64_t waves = ((int64_t)gx * chunks + at_once[i] - 1) / at_once[i];
-      const int warp_steps = (block_tiles + tw - 1) / tw * steps;
+      const int64_t blocks = (int64_t)gx * chunks, waves = blocks <= at_once[i] ? 1 : (blocks + at_once[i] - 1) / at_once[i];
+      const int warp_steps = ((block_tiles + tw - 1) >> j) * steps;
       // Microseconds.  A warp scheduler (it has every fourth warp) issues its warps' steps one after the other, or a warp's steps take their
       // latency; before that the tokens' rows are laid out by every block, after it threads add what the warps that split K have,
       // and ranks what the others have.  What it is for: 1 x 4096 x 4096 takes 4.7 us in blocks of two tile warps and 6.1 in
@@ -506,13 +506,13 @@ extern "C" int i4tc_w4a16_linear(const i4tc_w4a16_args* a, int device, void* str
       int issued = (block_tiles + 3) / 4 * each;
       if (tw < 4) {
         issued = 0;
-        for (int k = 0; k < k_warps; k += 4 / tw) issued += each > (k + 1) * steps ? steps : each > k * steps ? each - k * steps : 0;
-        issued *= (block_tiles + tw - 1) / tw;
+        for (int k = 0; k < k_warps; k += 4 >> j) issued += each > (k + 1) * steps ? steps : each > k * steps ? each - k * steps : 0;
+        issued *= (block_tiles + tw - 1) >> j;
       }
       const double issue = issued * (nt == 1 ? 0.143 : nt == 2 ? 0.2 : nt == 3 ? 0.278 : 0.333);
       const double latency = warp_steps * (0.3 + 0.01 * nt);
       const int rounds = (block_tiles * tokens * cols + kThreads - 1) / kThreads;
-      const double sums = (rounds + ranks - 1) / ranks * ((each + steps - 1) / steps) * 0.063;
+      const double sums = ((rounds + ranks - 1) >> i) * ((each + steps - 1) / steps) * 0.063;
       const double cost = waves * (0.7 + (issue > latency ? issue : latency) + each * tokens * 0.0034 + sums) + (ranks > 1 ? 1.5 + 0.07 * i : 0.0);
       if (grid_x == 0 || cost < best) {
         best = cost;
