@@ -676,7 +676,8 @@ def rope(x: torch.Tensor, positions: torch.Tensor, freqs: torch.Tensor, interlea
     """Rotary embedding of ``x`` [tokens, heads, D] (bf16 / fp16, any strides) at ``positions`` [tokens] (int32 / int64): the first
     ``2 * len(freqs)`` elements of every head turn by ``position * freqs`` (float64, of ``rope_frequencies``) and are multiplied by
     ``scale``, the rest is copied.  Pairs are ``(i, i + R/2)``, or ``(2i, 2i + 1)`` with ``interleaved``.  ``inverse`` turns back: it moves
-    keys to other positions, and is the gradient of ``rope``.  Angles are exact at any position; one rounding.  Returns a new
+    keys to other positions, and is the gradient of ``rope``.  Angles are computed in 64 bits, so that they are good to fp32 at any int32
+    position; one rounding.  Returns a new
     contiguous tensor."""
     return _rope(x, positions, freqs, interleaved, scale, inverse, False, "rope")
 
@@ -740,7 +741,8 @@ def kv_cache_append_(k_cache: torch.Tensor, v_cache: torch.Tensor, k: torch.Tens
     strides): row ``i < counts[b]`` (all T without ``counts``) becomes token ``lengths[b] + i`` of its sequence, in page
     ``block_table[b, token // page_size]``, and comes from new row ``select[b, i]`` (``i`` without ``select``): a prompt, or the accepted path
     of a tree of drafts.  All index tensors int32.  ``lengths`` stay as they are.  Counts, rows, tokens and pages out of range
-    write nothing and are raised by ``check_status``."""
+    write nothing and are raised by ``check_status``.  No two rows may go to one place, and none to a place that ``k`` and ``v`` are read from
+    (rows of the cache itself may be copied to other places of it)."""
     k, v, new, cache, block_table, lengths, index, sizes = _cache_pair(k_cache, v_cache, block_table, lengths, k, v)
     B, T = sizes[:2]
     counts_at = select_at = select_stride = 0
@@ -774,7 +776,7 @@ def tree_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: t
     A token that sees nothing gives zeros, and what a token does not see has no part in its result, infinities and NaN
     included.  ``scale`` defaults to D ** -0.5.  Scores, weights' sums and results are held in fp32; a weight is rounded to the
     values' type before it multiplies them, as the tensor cores take it, and summed as rounded.  Returns [B, T, heads, D].  Pages
-    and lengths out of range are raised by ``check_status``."""
+    and lengths out of range are raised by ``check_status``; the result of such a sequence means nothing, the others' stand."""
     kind = q.dtype
     code = _HALF.get(kind)
     if code is None or q.dim() != 4 or q.get_device() < 0 or (q.requires_grad and torch.is_grad_enabled()):

@@ -443,8 +443,10 @@ int i4tc_rope(const i4tc_rope_args* args, int device, void* stream);
  *   is row j % page_size of page block_table[b, j / page_size].
  * New token t sees the whole cache of its sequence and the new tokens j with mask[b, t, j] != 0 (bytes [tokens, tokens], mask_batch
  * apart, 0 for one that all share; NULL: j <= t).  A token that sees nothing gives zeros.  Strides in elements, multiples of 8
- * (queries: of 2); k and v share theirs, the caches share theirs.  At most 64 new tokens, D a multiple of 8 up to 128.  Lengths
- * beyond the table and pages out of range set bit 2 of the status word (i4tc_check_status), and read nothing.
+ * (queries: of 2); k and v share theirs, the caches share theirs.  At most 64 new tokens, D a multiple of 8 up to 128.  A length
+ * out of the table's range or a page out of range sets bit 2 of the status word (i4tc_check_status): the result of that
+ * sequence means nothing then, the others' stand, and nothing outside the operands is read.  block_table may be NULL with
+ * table_width 0 only, the caches with table_width or pages 0.
  * scratch: i4tc_tree_attention_scratch_bytes with most_length = table_width * page_size (0 for short tables: NULL will do); free
  * again when the call's work on its stream is done. */
 typedef struct {
@@ -464,7 +466,8 @@ int i4tc_tree_attention(const i4tc_tree_attention_args* args, int device, void* 
 /* Rows i < counts[b] (NULL: all `tokens`) of every sequence go into its cache as tokens lengths[b] + i, taken from new row
  * select[b, i] (int32, select_stride apart; NULL: i) of k and v [batch, tokens, kv_heads, D].  Cache, table and strides as above, of any
  * alignment.  Nothing else of the cache is written, and lengths stay as they are.  Counts, indices, tokens beyond the table
- * and pages out of range set bit 2 of the status word, and write nothing. */
+ * and pages out of range set bit 2 of the status word, and write nothing.  No two rows may go to one place, and none to a place that
+ * the call reads its rows from. */
 typedef struct {
   const void *k, *v;
   void *k_cache, *v_cache;
