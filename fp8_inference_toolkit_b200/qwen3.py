@@ -305,7 +305,8 @@ class Qwen3Prefill(nn.Module):
     def step(self, ids: torch.Tensor, cache: DecodeCache, tree_mask: torch.Tensor | None = None) -> torch.Tensor:
         """One token, a chain or a tree of drafts of every sequence: ids [B, T] -> final hidden states [B, T, hidden].  In a tree node t sees
         the nodes j with ``tree_mask[b, t, j]`` (bool, itself and its ancestors) and stands that many positions behind the cache.
-        ``cache.commit`` keeps the accepted ones; until then the cache is as it was, and the next ``step`` forgets them."""
+        ``cache.commit`` keeps the accepted ones; until then the cache is as it was, and the next ``step`` forgets them.  A captured graph
+        holds a step with its ``commit``: a replay leaves nothing to commit."""
         cache.pending, made = [], []     # a step that raises half-way leaves nothing to commit
         B, T = ids.shape
         freqs = cache.freqs
