@@ -107,8 +107,8 @@ class Block(nn.Module):
         self.ln2 = RMSNorm(cfg.hidden, cfg.eps, device)
         self.q_norm = RMSNorm(cfg.head_dim, cfg.eps, device)
         self.k_norm = RMSNorm(cfg.head_dim, cfg.eps, device)
-        # fold the quantisers into RMSNorm / SwiGLU (per-group scales only; the per-channel ops and 16-bit activations keep the plain path)
-        self.fused = fused and not per_channel and self.qkv.method.act_bits == 4
+        # fold the quantisers into RMSNorm / SwiGLU (per-group scales only; the per-channel ops keep the plain path)
+        self.fused = fused and not per_channel
 
     @staticmethod
     def _lin(k, n, device, per_channel, gen):
@@ -122,7 +122,8 @@ class Block(nn.Module):
     def forward(self, x, cos, sin, attend=None):
         cfg = self.cfg
         B, S, _ = x.shape
-        if self.fused and _bare(self.qkv, self.gate_up, self.down):
+        folded = self.qkv, self.gate_up, self.down     # (as they are now: a layer may have been given others)
+        if self.fused and _bare(*folded) and all(lin.method.act_bits == 4 for lin in folded):
             return self._forward_fused(x, cos, sin, attend)
         qkv = self.qkv(self.ln1(x))
         if attend is not None:

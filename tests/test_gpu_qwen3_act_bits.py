@@ -38,3 +38,17 @@ def test_prompts_follow_the_flag(bits, monkeypatch):
     else:
         assert quantised > 0 and calls["w4a16_linear"] == 0
     ops.check_status()
+
+
+@pytest.mark.parametrize("name", ["qkv", "gate_up", "down"])
+def test_a_layer_given_a_linear_of_16_bits(name, monkeypatch):
+    """A layer's own way is that of the linears it has, not of those it was built with."""
+    from fp8_inference_toolkit_b200 import ops
+    from fp8_inference_toolkit_b200.qwen3 import Qwen3Config, Qwen3Prefill
+
+    cfg = Qwen3Config(hidden=1024, layers=1, q_heads=8, kv_heads=2, head_dim=128, inter=1536, vocab=64)
+    model = Qwen3Prefill(cfg)
+    getattr(model.blocks[0], name).method.act_bits = 16
+    calls, op = [], ops.w4a16_linear
+    monkeypatch.setattr(ops, "w4a16_linear", lambda *a: calls.append(1) or op(*a))
+    assert model(torch.arange(9, device="cuda").view(1, 9)).isfinite().all() and len(calls) == 1
